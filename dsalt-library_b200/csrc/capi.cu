@@ -3,7 +3,7 @@
 #include <cudaTypedefs.h>
 #include <mutex>
 
-#include "common.cuh"
+#include "ffn.cuh"
 #include "sm100.cuh"
 
 namespace dsalt {
@@ -44,6 +44,9 @@ cudaError_t launch_swiglu(const DsaltSwigluParams& p, bool bwd, cudaStream_t st)
 cudaError_t launch_win_gate_bwd(const DsaltWinGateBwdParams& p, cudaStream_t st);
 cudaError_t launch_hybrid_scores_bwd(const DsaltScoreBwdParams& p, cudaStream_t st);
 cudaError_t launch_gqa_reduce(const DsaltGqaReduceParams& p, cudaStream_t st);
+cudaError_t launch_dropout(const DsaltDropoutParams& p, cudaStream_t st);
+cudaError_t launch_residual_norm(const DsaltResidualNormParams& p, bool bwd, cudaStream_t st);
+cudaError_t residual_norm_parts(int64_t T, int d, int* out);
 cudaError_t launch_wait_timeout_probe(int32_t* status, cudaStream_t st);
 cudaError_t launch_hybrid_scores(const DsaltScoreParams& p, cudaStream_t st);
 cudaError_t launch_topk(const DsaltTopkParams& p, cudaStream_t st);
@@ -153,6 +156,9 @@ int dsalt_b200_params_sizeof(int which) {
     case 11: return (int)sizeof(DsaltWinGateBwdParams);
     case 12: return (int)sizeof(DsaltScoreBwdParams);
     case 13: return (int)sizeof(DsaltGqaReduceParams);
+    case 14: return (int)sizeof(DsaltGatedFfnParams);
+    case 15: return (int)sizeof(DsaltDropoutParams);
+    case 16: return (int)sizeof(DsaltResidualNormParams);
   }
   return -1;
 }
@@ -388,6 +394,120 @@ int dsalt_gqa_reduce(const DsaltGqaReduceParams* p, void* stream) {
   if (!p->x || !p->y) return DSALT_ERR_ARG;
   if (!aligned16(p->x) || !aligned16(p->y)) return DSALT_ERR_ALIGN;
   return status_of(launch_gqa_reduce(*p, (cudaStream_t)stream));
+}
+
+// Sizes and the operands that a stage reads and writes; every stride covers its row.
+static int check_ffn(const DsaltGatedFfnParams* p, int stage) {
+  if (!p || p->T < 0 || p->d <= 0 || p->F <= 0 || p->d_out <= 0) return DSALT_ERR_ARG;
+  if (p->dtype != DSALT_F16 && p->dtype != DSALT_BF16) return DSALT_ERR_DTYPE;
+  if (p->activation < DSALT_ACT_SILU || p->activation > DSALT_ACT_GELU_TANH) return DSALT_ERR_ARG;
+  // tile coordinates and counts are 32-bit
+  const int64_t most = (int64_t)1 << 30;
+  if (p->T > most || p->d > most || p->F > most || p->d_out > most) return DSALT_ERR_TOO_LARGE;
+  const int64_t tall = p->T > p->F ? p->T : p->F, wide = p->d > p->d_out ? p->d : p->d_out;
+  const int64_t cols = p->F > wide ? p->F : wide, rows = tall > wide ? tall : wide;
+  if (((rows + 127) / 128) * ((cols + 127) / 128) > INT32_MAX / 4) return DSALT_ERR_TOO_LARGE;
+  struct In { const void* ptr; int64_t ld, width; };
+  const In x = {p->x, p->ld_x, p->d}, wg = {p->w_gate, p->ld_wg, p->d}, wu = {p->w_up, p->ld_wu, p->d},
+           wd = {p->w_down, p->ld_wd, p->F}, dy = {p->dy, p->ld_dy, p->d_out}, h = {p->h, p->ld_f, p->F},
+           a = {p->a, p->ld_f, p->F}, b = {p->b, p->ld_f, p->F}, dg = {p->dg, p->ld_f, p->F}, du = {p->du, p->ld_f, p->F};
+  In need[6];
+  int n = 0;
+  switch (stage) {
+    case FFN_HIDDEN:
+      if ((p->a == nullptr) != (p->b == nullptr)) return DSALT_ERR_ARG;
+      need[n++] = x; need[n++] = wg; need[n++] = wu; need[n++] = h;
+      if (p->a) { need[n++] = a; need[n++] = b; }
+      break;
+    case FFN_OUT: need[n++] = h; need[n++] = wd; break;
+    case FFN_BWD_HIDDEN: need[n++] = dy; need[n++] = wd; need[n++] = a; need[n++] = b; need[n++] = dg; need[n++] = du; break;
+    case FFN_BWD_INPUT: need[n++] = dg; need[n++] = du; need[n++] = wg; need[n++] = wu; break;
+    default:
+      if (p->dw_gate) need[n++] = dg;
+      if (p->dw_up) need[n++] = du;
+      if (p->dw_gate || p->dw_up) need[n++] = x;
+      if (p->dw_down) { need[n++] = dy; need[n++] = h; }
+  }
+  for (int i = 0; i < n; ++i)
+    if (need[i].ld < need[i].width || need[i].ld % 8 != 0 || need[i].ld > ((int64_t)1 << 38)) return DSALT_ERR_ARG;
+  if (p->T == 0) return DSALT_OK;
+  for (int i = 0; i < n; ++i) {
+    if (!need[i].ptr) return DSALT_ERR_ARG;
+    if (!aligned16(need[i].ptr)) return DSALT_ERR_ALIGN;
+  }
+  if ((stage == FFN_OUT && !p->y) || (stage == FFN_BWD_INPUT && !p->dx)) return DSALT_ERR_ARG;
+  return DSALT_OK;
+}
+
+static int run_ffn(const DsaltGatedFfnParams* p, int stage, void* stream) {
+  const int rc = check_ffn(p, stage);
+  if (rc != DSALT_OK) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (p->T > 0) return status_of(launch_ffn(stage, *p, st));
+  if (stage != FFN_BWD_WEIGHTS) return DSALT_OK;
+  // no tokens: the weight gradients are 0
+  const size_t es = p->w_grad_f32 ? 4 : 2;
+  cudaError_t e = cudaSuccess;
+  if (p->dw_gate) e = cudaMemsetAsync(p->dw_gate, 0, (size_t)p->F * p->d * es, st);
+  if (e == cudaSuccess && p->dw_up) e = cudaMemsetAsync(p->dw_up, 0, (size_t)p->F * p->d * es, st);
+  if (e == cudaSuccess && p->dw_down) e = cudaMemsetAsync(p->dw_down, 0, (size_t)p->d_out * p->F * es, st);
+  return status_of(e);
+}
+
+int dsalt_gated_ffn_hidden(const DsaltGatedFfnParams* p, void* stream) { return run_ffn(p, FFN_HIDDEN, stream); }
+int dsalt_gated_ffn_out(const DsaltGatedFfnParams* p, void* stream) { return run_ffn(p, FFN_OUT, stream); }
+int dsalt_gated_ffn_bwd_hidden(const DsaltGatedFfnParams* p, void* stream) { return run_ffn(p, FFN_BWD_HIDDEN, stream); }
+int dsalt_gated_ffn_bwd_input(const DsaltGatedFfnParams* p, void* stream) { return run_ffn(p, FFN_BWD_INPUT, stream); }
+int dsalt_gated_ffn_bwd_weights(const DsaltGatedFfnParams* p, void* stream) { return run_ffn(p, FFN_BWD_WEIGHTS, stream); }
+
+int dsalt_dropout(const DsaltDropoutParams* p, void* stream) {
+  if (!p || p->n < 0 || p->threshold < 0 || p->threshold > 65536) return DSALT_ERR_ARG;
+  if (p->dtype != DSALT_F16 && p->dtype != DSALT_BF16 && p->dtype != DSALT_F32) return DSALT_ERR_DTYPE;
+  if (p->n > (int64_t)1 << 41) return DSALT_ERR_TOO_LARGE;
+  if (p->n == 0) return DSALT_OK;
+  if (!p->x || !p->y || (p->threshold > 0 && !p->seed)) return DSALT_ERR_ARG;
+  return status_of(launch_dropout(*p, (cudaStream_t)stream));
+}
+
+static int check_residual(const DsaltResidualNormParams* p, bool bwd) {
+  if (!p || p->T < 0 || p->d <= 0 || !(p->eps >= 0.f)) return DSALT_ERR_ARG;
+  if (p->dtype != DSALT_F16 && p->dtype != DSALT_BF16 && p->dtype != DSALT_F32) return DSALT_ERR_DTYPE;
+  if (p->threshold < 0 || p->threshold > 65536) return DSALT_ERR_ARG;
+  if (p->gate_mode < DSALT_GATE_NONE || p->gate_mode > DSALT_GATE_FULL) return DSALT_ERR_ARG;
+  if (p->d > DSALT_RESIDUAL_MAX_D || p->T > ((int64_t)1 << 46) / p->d) return DSALT_ERR_TOO_LARGE;
+  if (p->T == 0) return DSALT_OK;
+  if (!p->f || !p->x_new || (p->threshold > 0 && !p->seed)) return DSALT_ERR_ARG;
+  if (p->gate_mode != DSALT_GATE_NONE && !p->gate) return DSALT_ERR_ARG;
+  if (!bwd) return p->x && (!p->norm || p->h) ? DSALT_OK : DSALT_ERR_ARG;
+  if (!p->dx || !p->df || !p->parts || (p->gate_mode != DSALT_GATE_NONE && !p->dgate)) return DSALT_ERR_ARG;
+  if ((p->post && !p->rf) || (p->norm && p->dh && !p->r)) return DSALT_ERR_ARG;
+  return DSALT_OK;
+}
+
+int dsalt_residual_norm_fwd(const DsaltResidualNormParams* p, void* stream) {
+  const int rc = check_residual(p, false);
+  if (rc != DSALT_OK || p->T == 0) return rc;
+  return status_of(launch_residual_norm(*p, false, (cudaStream_t)stream));
+}
+
+int dsalt_residual_norm_bwd(const DsaltResidualNormParams* p, void* stream) {
+  const int rc = check_residual(p, true);
+  if (rc != DSALT_OK) return rc;
+  if (p->T > 0) return status_of(launch_residual_norm(*p, true, (cudaStream_t)stream));
+  // no rows: the sums over them are 0
+  const size_t es = p->w_f32 || p->dtype == DSALT_F32 ? 4 : 2;
+  cudaError_t e = cudaSuccess;
+  for (void* out : {p->dscale, p->dpost, p->dnorm})
+    if (e == cudaSuccess && out) e = cudaMemsetAsync(out, 0, (size_t)p->d * es, (cudaStream_t)stream);
+  return status_of(e);
+}
+
+int dsalt_residual_norm_parts(int64_t T, int32_t d) {
+  if (T < 0 || d <= 0) return -DSALT_ERR_ARG;
+  if (d > DSALT_RESIDUAL_MAX_D) return -DSALT_ERR_TOO_LARGE;
+  int n = 0;
+  const int rc = status_of(residual_norm_parts(T, d, &n));
+  return rc == DSALT_OK ? n : -rc;
 }
 
 }  // extern "C"

@@ -21,7 +21,7 @@ F16, BF16, F32 = 0, 1, 2
 TRAIN, INFER = 0, 1
 IMPL_AUTO, IMPL_SIMT, IMPL_TCGEN05 = 0, 1, 2
 DEV_WAIT_TIMEOUT, DEV_BAD_INDEX = 1, 2
-ABI_VERSION = 8
+ABI_VERSION = 9
 QREC_FLOATS = 16  # DSALT_QREC_FLOATS
 LMK_SPLIT = 4  # DSALT_LMK_SPLIT
 DS_TILE_BYTES = 16384  # DSALT_DS_TILE_BYTES
@@ -140,9 +140,37 @@ class GqaReduceParams(ctypes.Structure):
                 ("dtype", _i32)]
 
 
+class GatedFfnParams(ctypes.Structure):
+    _fields_ = [("x", _c_void_p), ("w_gate", _c_void_p), ("w_up", _c_void_p), ("w_down", _c_void_p),
+                ("h", _c_void_p), ("a", _c_void_p), ("b", _c_void_p), ("y", _c_void_p), ("dy", _c_void_p),
+                ("dg", _c_void_p), ("du", _c_void_p), ("dx", _c_void_p), ("dw_gate", _c_void_p),
+                ("dw_up", _c_void_p), ("dw_down", _c_void_p), ("status", _c_void_p), ("T", _i64),
+                ("ld_x", _i64), ("ld_wg", _i64), ("ld_wu", _i64), ("ld_wd", _i64), ("ld_f", _i64), ("ld_dy", _i64),
+                ("d", _i32), ("F", _i32), ("d_out", _i32), ("activation", _i32), ("dtype", _i32),
+                ("w_grad_f32", _i32)]
+
+
+class DropoutParams(ctypes.Structure):
+    _fields_ = [("x", _c_void_p), ("y", _c_void_p), ("seed", _c_void_p), ("n", _i64), ("site", ctypes.c_uint32),
+                ("threshold", _i32), ("dtype", _i32)]
+
+
+class ResidualNormParams(ctypes.Structure):
+    _fields_ = [("x", _c_void_p), ("f", _c_void_p), ("gate", _c_void_p), ("post", _c_void_p), ("scale", _c_void_p),
+                ("norm", _c_void_p), ("x_new", _c_void_p), ("h", _c_void_p), ("rf", _c_void_p), ("r", _c_void_p),
+                ("dx_new", _c_void_p), ("dh", _c_void_p), ("dx", _c_void_p), ("df", _c_void_p),
+                ("dgate", _c_void_p), ("dpost", _c_void_p), ("dscale", _c_void_p), ("dnorm", _c_void_p),
+                ("parts", _c_void_p), ("seed", _c_void_p), ("T", _i64), ("d", _i32), ("eps", _f32),
+                ("site", ctypes.c_uint32), ("threshold", _i32), ("gate_mode", _i32), ("dtype", _i32),
+                ("w_f32", _i32)]
+
+
+GATE_NONE, GATE_TOKEN, GATE_FULL = 0, 1, 2  # DSALT_GATE_*
+RESIDUAL_MAX_D = 16384  # DSALT_RESIDUAL_MAX_D
+
 _STRUCTS = [ScheduleParams, GatherParams, AttnParams, ScoreParams, TopkParams, WinGateParams, RopeParams,
             RmsNormParams, ScaleRowsParams, XentParams, SwigluParams, WinGateBwdParams, ScoreBwdParams,
-            GqaReduceParams]
+            GqaReduceParams, GatedFfnParams, DropoutParams, ResidualNormParams]
 _ENTRY = {
     "dsalt_build_schedule": ScheduleParams,
     "dsalt_gather_landmarks": GatherParams,
@@ -165,6 +193,14 @@ _ENTRY = {
     "dsalt_swiglu_fwd": SwigluParams,
     "dsalt_swiglu_bwd": SwigluParams,
     "dsalt_gqa_reduce": GqaReduceParams,
+    "dsalt_gated_ffn_hidden": GatedFfnParams,
+    "dsalt_gated_ffn_out": GatedFfnParams,
+    "dsalt_gated_ffn_bwd_hidden": GatedFfnParams,
+    "dsalt_gated_ffn_bwd_input": GatedFfnParams,
+    "dsalt_gated_ffn_bwd_weights": GatedFfnParams,
+    "dsalt_dropout": DropoutParams,
+    "dsalt_residual_norm_fwd": ResidualNormParams,
+    "dsalt_residual_norm_bwd": ResidualNormParams,
 }
 
 _lib = None
@@ -196,6 +232,8 @@ def load() -> ctypes.CDLL:
         n = lib.dsalt_b200_params_sizeof(i)
         if n != ctypes.sizeof(st):
             raise RuntimeError(f"{st.__name__}: ctypes size {ctypes.sizeof(st)} != C size {n}")
+    lib.dsalt_residual_norm_parts.restype = ctypes.c_int
+    lib.dsalt_residual_norm_parts.argtypes = [_i64, _i32]
     for name, st in _ENTRY.items():
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
@@ -234,6 +272,25 @@ def call(name: str, params) -> None:
     if rec is not None:
         e1.record(cs)
         rec.append((name, e0, e1))
+
+
+def call_on(device: torch.device, names, params) -> None:
+    """``call`` each of ``names`` with the same parameters on the current stream of
+    ``device``, which need not be the current device."""
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        for name in names:
+            call(name, params)
+        return
+    with torch.cuda.device(device):
+        for name in names:
+            call(name, params)
+
+
+def same_device(device: torch.device, **tensors) -> None:
+    """Raise unless every given tensor (None is skipped) is on ``device``."""
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
 def ptr(t) -> int:

@@ -1,0 +1,147 @@
+"""Gated feed-forward block on the library's own tensor-core kernels.
+
+``gated_ffn(x, w_gate, w_up, w_down)`` is ``down(act(gate(x)) * up(x))``, the block
+of ``dsalt/modules/dsalt_transformer.py:10-21`` (``act`` = silu there), in f16 or
+bf16 with fp32 accumulation.  Both projections, the activation and the product are
+one kernel: neither ``gate(x)`` nor ``up(x)`` is written to memory.  A forward that
+needs gradients also keeps ``a = act(g)`` and ``b = u·act'(g)``, from which the
+backward forms ``du = dh·a`` and ``dg = dh·b`` in the epilogue of the product that
+makes ``dh``.  Results are rounded once from the fp32 sums; only ``h`` (the operand
+of the second product) and, in the backward, ``a``, ``b``, ``dg`` and ``du`` are
+rounded on the way.
+
+``swiglu_ffn`` computes the same block with library GEMMs around an activation
+kernel, with torch's rounding at every step.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _ext
+from .dsalt_cuda import device_status
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}  # DSALT_ACT_*
+
+
+def _operand(t: torch.Tensor, dtype: torch.dtype):
+    """``(tensor, row stride)`` of a 2-D operand as the kernels read it: ``t`` itself when
+    its rows are contiguous, 16-byte aligned and apart, else a copy that is."""
+    rows, cols = t.shape
+    if t.dtype == dtype and t.stride(1) == 1 and t.data_ptr() % 16 == 0:
+        if rows == 1:
+            return t, (cols + 7) // 8 * 8
+        if t.stride(0) % 8 == 0 and t.stride(0) >= cols:
+            return t, t.stride(0)
+    ld = (cols + 7) // 8 * 8
+    buf = torch.empty(rows, ld, dtype=dtype, device=t.device)
+    buf[:, :cols].copy_(t)
+    return buf[:, :cols], ld
+
+
+def _params(x2, wg, wu, wd, activation: int, dtype: torch.dtype):
+    (x_, ld_x), (wg_, ld_wg), (wu_, ld_wu), (wd_, ld_wd) = x2, wg, wu, wd
+    F, d = wg_.shape
+    return _ext.GatedFfnParams(x=x_.data_ptr(), w_gate=wg_.data_ptr(), w_up=wu_.data_ptr(), w_down=wd_.data_ptr(),
+                               status=device_status(x_.device).data_ptr(), T=x_.shape[0], ld_x=ld_x, ld_wg=ld_wg,
+                               ld_wu=ld_wu, ld_wd=ld_wd, ld_f=(F + 7) // 8 * 8, d=d, F=F, d_out=wd_.shape[0],
+                               activation=activation, dtype=_ext.dtype_code(dtype))
+
+
+def _forward(x2, wg, wu, wd, activation: int, dtype: torch.dtype, keep: bool):
+    """``(y, h, a, b)``; ``a`` and ``b`` only with ``keep``."""
+    p = _params(x2, wg, wu, wd, activation, dtype)
+    dev = x2[0].device
+    h, a, b = (torch.empty(p.T, p.ld_f, dtype=dtype, device=dev) if i == 0 or keep else None for i in range(3))
+    y = torch.empty(p.T, p.d_out, dtype=dtype, device=dev)
+    p.h, p.a, p.b, p.y = h.data_ptr(), _ext.ptr(a), _ext.ptr(b), y.data_ptr()
+    _ext.call_on(dev, ("dsalt_gated_ffn_hidden", "dsalt_gated_ffn_out"), p)
+    return y, h, a, b
+
+
+class GatedFFNFunction(torch.autograd.Function):
+    """``(x [T, d], w_gate [F, d], w_up [F, d], w_down [d_out, F], activation, dtype) -> [T, d_out]``."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, activation: int, dtype: torch.dtype):
+        ops = [_operand(t.detach(), dtype) for t in (x, w_gate, w_up, w_down)]
+        y, h, a, b = _forward(*ops, activation, dtype, True)
+        ctx.save_for_backward(*(t for t, _ in ops), h, a, b)
+        ctx.strides = [ld for _, ld in ops]
+        ctx.activation, ctx.dtype = activation, dtype
+        ctx.dtypes = [t.dtype for t in (x, w_gate, w_up, w_down)]
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        *ops, h, a, b = ctx.saved_tensors
+        dtype, dev = ctx.dtype, h.device
+        p = _params(*zip(ops, ctx.strides), ctx.activation, dtype)
+        dy_, p.ld_dy = _operand(dy, dtype)
+        need_x, *need_w = ctx.needs_input_grad[:4]
+        p.h, p.a, p.b, p.dy = h.data_ptr(), a.data_ptr(), b.data_ptr(), dy_.data_ptr()
+        stages = []
+        if need_x or need_w[0] or need_w[1]:
+            dg, du = torch.empty_like(a), torch.empty_like(a)
+            p.dg, p.du = dg.data_ptr(), du.data_ptr()
+            stages.append("dsalt_gated_ffn_bwd_hidden")
+        grads = [None] * 4
+        if need_x:
+            grads[0] = torch.empty(p.T, p.d, dtype=dtype, device=dev)
+            p.dx = grads[0].data_ptr()
+            stages.append("dsalt_gated_ffn_bwd_input")
+        if any(need_w):
+            # fp32 sums where a weight is not of the compute dtype: its gradient is rounded once
+            p.w_grad_f32 = int(any(dt != dtype for dt in ctx.dtypes[1:]))
+            out = torch.float32 if p.w_grad_f32 else dtype
+            shapes = ((p.F, p.d), (p.F, p.d), (p.d_out, p.F))
+            for i, (need, shape) in enumerate(zip(need_w, shapes)):
+                if need:
+                    grads[1 + i] = torch.empty(shape, dtype=out, device=dev)
+            p.dw_gate, p.dw_up, p.dw_down = (_ext.ptr(t) for t in grads[1:])
+            stages.append("dsalt_gated_ffn_bwd_weights")
+        _ext.call_on(dev, stages, p)
+        return (*(t if t is None else t.to(dt) for t, dt in zip(grads, ctx.dtypes)), None, None)
+
+
+def _check(x, w_gate, w_up, w_down, activation):
+    _ext.require_cuda(x, "x")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+    if x.dim() == 0 or w_gate.dim() != 2 or w_up.dim() != 2 or w_down.dim() != 2:
+        raise ValueError("gated_ffn takes x [..., d], w_gate and w_up [F, d], w_down [d_out, F]")
+    F, d = w_gate.shape
+    if x.shape[-1] != d or w_up.shape != w_gate.shape or w_down.shape[1] != F:
+        raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, "
+                         f"w_up {tuple(w_up.shape)}, w_down {tuple(w_down.shape)}")
+    if F == 0 or d == 0 or w_down.shape[0] == 0:
+        raise ValueError("gated_ffn needs widths of at least 1")
+    _ext.same_device(x.device, w_gate=w_gate, w_up=w_up, w_down=w_down)
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+              activation: str = "silu", dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``(act(x w_gateᵀ) * (x w_upᵀ)) w_downᵀ``, ``[..., d] -> [..., d_out]``, in f16 or bf16.
+
+    ``activation``: ``"silu"``, ``"gelu"`` (erf) or ``"gelu_tanh"``.  ``dtype`` is the
+    compute dtype; by default autocast's, or the one 16-bit dtype of all four tensors.
+    Tensors of other dtypes are cast to it and get gradients of their own dtype.
+    Operands are read in place when their rows are contiguous and 16-byte aligned
+    (a slice of a stacked weight is), else copied first.  First derivatives only.
+    """
+    _check(x, w_gate, w_up, w_down, activation)
+    if dtype is None:
+        dtype = _ext.half_compute_dtype(x, w_gate, w_up, w_down)
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("gated_ffn computes in float16 or bfloat16: pass 16-bit tensors of one dtype, use autocast "
+                        f"or give dtype (got x {x.dtype}, w_gate {w_gate.dtype}, dtype {dtype})")
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    act = ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
+                                    or w_down.requires_grad):
+        y = GatedFFNFunction.apply(x2, w_gate, w_up, w_down, act, dtype)
+    else:
+        y = _forward(*(_operand(t, dtype) for t in (x2, w_gate, w_up, w_down)), act, dtype, False)[0]
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])

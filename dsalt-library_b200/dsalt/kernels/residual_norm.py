@@ -1,0 +1,144 @@
+"""From one block to the next in one kernel each way: the norm after a block, its
+gate and residual scale, dropout, the residual add and the norm before the next
+block (``dsalt_residual_norm_fwd`` / ``_bwd`` in ``csrc/residual_norm.cu``).
+
+``rmsnorm_cuda.add_rms_norm`` is the add and the second norm alone, for four widths.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _ext
+from .counter_dropout import check_seed, drop_threshold
+
+
+def _vectors(dtype: torch.dtype, *vs):
+    """The given weight vectors as the kernels read them (all of ``dtype``, or all fp32) and which."""
+    given = [v for v in vs if v is not None]
+    f32 = any(v.dtype != dtype for v in given)
+    want = torch.float32 if f32 else dtype
+    return [None if v is None else v.detach().to(want).contiguous() for v in vs], f32
+
+
+def _params(x_new, f, gate, vectors, f32, seed, eps, site, threshold, gate_mode):
+    post, scale, norm = vectors
+    return _ext.ResidualNormParams(f=f.data_ptr(), gate=_ext.ptr(gate), post=_ext.ptr(post), scale=_ext.ptr(scale),
+                                   norm=_ext.ptr(norm), x_new=x_new.data_ptr(), seed=_ext.ptr(seed), T=f.shape[0],
+                                   d=f.shape[1], eps=eps, site=site, threshold=threshold, gate_mode=gate_mode,
+                                   dtype=_ext.dtype_code(f.dtype), w_f32=int(f32))
+
+
+def _forward(x, f, gate, vectors, f32, seed, eps, site, threshold, gate_mode, keep: bool):
+    """``(x_new, h, rf, r)``; the inverse root mean squares only with ``keep``."""
+    post, _, norm = vectors
+    x_new = torch.empty_like(f)
+    h = torch.empty_like(f) if norm is not None else None
+    p = _params(x_new, f, gate, vectors, f32, seed, eps, site, threshold, gate_mode)
+    rf = torch.empty(p.T, dtype=torch.float32, device=f.device) if keep and post is not None else None
+    r = torch.empty(p.T, dtype=torch.float32, device=f.device) if keep and norm is not None else None
+    p.x, p.h, p.rf, p.r = x.data_ptr(), _ext.ptr(h), _ext.ptr(rf), _ext.ptr(r)
+    _ext.call_on(f.device, ("dsalt_residual_norm_fwd",), p)
+    return x_new, h, rf, r
+
+
+class ResidualNormFunction(torch.autograd.Function):
+    """``(x, f, post, scale, gate, norm, seed, eps, site, threshold, gate_mode) -> (x_new, h)``
+    on ``[T, d]``; without ``norm`` only ``x_new``."""
+
+    @staticmethod
+    def forward(ctx, x, f, post, scale, gate, norm, seed, eps, site, threshold, gate_mode):
+        x, f = x.detach().contiguous(), f.detach().contiguous()
+        g = None if gate is None else gate.detach().contiguous()
+        vectors, f32 = _vectors(f.dtype, post, scale, norm)
+        x_new, h, rf, r = _forward(x, f, g, vectors, f32, seed, eps, site, threshold, gate_mode, True)
+        ctx.save_for_backward(x_new, f, g, *vectors, seed, rf, r)
+        ctx.scalars = (eps, site, threshold, gate_mode)
+        ctx.f32 = f32
+        ctx.dtypes = [None if v is None else v.dtype for v in (post, scale, norm)]
+        ctx.set_materialize_grads(False)
+        return x_new if h is None else (x_new, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dx_new, dh=None):
+        x_new, f, gate, post, scale, norm, seed, rf, r = ctx.saved_tensors
+        p = _params(x_new, f, gate, (post, scale, norm), ctx.f32, seed, *ctx.scalars)
+        dx_new, dh = (None if t is None else t.contiguous() for t in (dx_new, dh))
+        dx, df = torch.empty_like(f), torch.empty_like(f)
+        dgate = None if gate is None else torch.empty_like(gate)
+        need = (ctx.needs_input_grad[2], ctx.needs_input_grad[3], ctx.needs_input_grad[5])
+        dpost, dscale, dnorm = (torch.empty_like(v) if v is not None and n else None
+                                for v, n in zip((post, scale, norm), need))
+        with torch.cuda.device(f.device):
+            n = _ext.load().dsalt_residual_norm_parts(p.T, p.d)
+        if n < 0:
+            raise RuntimeError(f"dsalt_residual_norm_parts failed: {_ext.status_string(-n)}")
+        parts = torch.empty(max(n, 1), 3, p.d, dtype=torch.float32, device=f.device)
+        p.rf, p.r, p.dx_new, p.dh = _ext.ptr(rf), _ext.ptr(r), _ext.ptr(dx_new), _ext.ptr(dh)
+        p.dx, p.df, p.dgate, p.parts = dx.data_ptr(), df.data_ptr(), _ext.ptr(dgate), parts.data_ptr()
+        p.dpost, p.dscale, p.dnorm = _ext.ptr(dpost), _ext.ptr(dscale), _ext.ptr(dnorm)
+        _ext.call_on(f.device, ("dsalt_residual_norm_bwd",), p)
+        dpost, dscale, dnorm = (t if t is None else t.to(dt) for t, dt in zip((dpost, dscale, dnorm), ctx.dtypes))
+        return dx, df, dpost, dscale, dgate, dnorm, None, None, None, None, None
+
+
+def residual_norm(x: torch.Tensor, f: torch.Tensor, norm_weight: torch.Tensor | None = None, *,
+                  post_weight: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+                  gate: torch.Tensor | None = None, dropout_p: float = 0.0, seed: torch.Tensor | None = None,
+                  site: int = 0, eps: float = 1e-6):
+    """``(x_new, h)``: ``x_new = x + drop(scale * gate * norm(f))`` and ``h = norm(x_new)``.
+
+    ``x`` (the residual stream) and ``f`` (a block's output): ``[..., d]`` of one dtype
+    (f16, bf16, f32).  ``post_weight``, ``scale``, ``norm_weight``: ``[d]``, each may be left
+    out: no norm of ``f``, no scale, no second norm (``h`` is then None).  ``gate``: x's
+    dtype, one value per token (``[...]`` or ``[..., 1]``) or per element (``[..., d]``).
+    Dropout draws as ``counter_dropout`` does for a tensor of x's shape.  ``h`` is the
+    norm of the rounded ``x_new``.  All sums are fp32.  First derivatives only; the
+    gradients of the vectors are summed in a fixed order.
+    """
+    _ext.require_cuda(x, "x")
+    _ext.dtype_code(x.dtype)
+    if x.dim() == 0 or f.shape != x.shape or f.dtype != x.dtype:
+        raise ValueError(f"x and f must have one shape [..., d] and dtype, got {tuple(x.shape)} {x.dtype} and "
+                         f"{tuple(f.shape)} {f.dtype}")
+    d = x.shape[-1]
+    if not 1 <= d <= _ext.RESIDUAL_MAX_D:
+        raise ValueError(f"d must be in [1, {_ext.RESIDUAL_MAX_D}], got {d}")
+    for name, v in (("post_weight", post_weight), ("scale", scale), ("norm_weight", norm_weight)):
+        if v is not None and (v.shape != (d,) or not v.is_floating_point()):
+            raise ValueError(f"{name} must be a floating vector of {d} elements, got {tuple(v.shape)} {v.dtype}")
+    gate_mode = _ext.GATE_NONE
+    if gate is not None:
+        if gate.dtype != x.dtype:
+            raise ValueError(f"gate must have x's dtype {x.dtype}, got {gate.dtype}")
+        if gate.shape == x.shape:
+            gate_mode = _ext.GATE_FULL
+        elif gate.shape == x.shape[:-1] or gate.shape == (*x.shape[:-1], 1):
+            gate_mode = _ext.GATE_TOKEN
+        else:
+            raise ValueError(f"gate must have one value per token or element of x {tuple(x.shape)}, "
+                             f"got {tuple(gate.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    threshold = drop_threshold(dropout_p)
+    if threshold > 0:
+        check_seed(seed, site, x.device)
+    else:
+        seed, site = None, 0
+    _ext.same_device(x.device, f=f, post_weight=post_weight, scale=scale, gate=gate, norm_weight=norm_weight)
+    x2, f2 = (t if t.dim() == 2 else t.reshape(-1, d) for t in (x, f))
+    leaves = (x, f, post_weight, scale, gate, norm_weight)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves):
+        out = ResidualNormFunction.apply(x2, f2, post_weight, scale, gate, norm_weight, seed, float(eps), site,
+                                         threshold, gate_mode)
+        x_new, h = out if norm_weight is not None else (out, None)
+    else:
+        vectors, f32 = _vectors(x.dtype, post_weight, scale, norm_weight)
+        g = None if gate is None else gate.contiguous()
+        x_new, h, _, _ = _forward(x2.contiguous(), f2.contiguous(), g, vectors, f32, seed, float(eps), site, threshold,
+                                  gate_mode, False)
+    if x.dim() != 2:
+        x_new, h = x_new.view(x.shape), None if h is None else h.view(x.shape)
+    return x_new, h

@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define DSALT_B200_ABI_VERSION 8
+#define DSALT_B200_ABI_VERSION 9
 
 /* The tensor-core dK/dV stage splits each landmark chunk's query range into
  * this many parts that run as separate CTAs; their fp32 partial sums are added
@@ -491,6 +491,117 @@ typedef struct DsaltSwigluParams {
 DSALT_API int dsalt_swiglu_fwd(const DsaltSwigluParams* p, void* stream);
 DSALT_API int dsalt_swiglu_bwd(const DsaltSwigluParams* p, void* stream);
 
+/* Gated feed-forward block, f16 / bf16, fp32 accumulation:
+ *   g = x·Wgᵀ, u = x·Wuᵀ, h = act(g)⊙u, y = h·Wdᵀ
+ * (dsalt/modules/dsalt_transformer.py:10-21 with act = silu), as five stages that
+ * read their operands in place (row-major, row strides ld_*):
+ *   hidden       h, and for a later backward a = act(g), b = u⊙act'(g) (both or
+ *                neither), each rounded once from fp32; g and u are not stored
+ *   out          y
+ *   bwd_hidden   dh = dy·Wd (kept in fp32), du = R(dh⊙a), dg = R(dh⊙b)
+ *   bwd_input    dx = R(dg·Wg + du·Wu), one accumulation
+ *   bwd_weights  dWg = dgᵀ·x, dWu = duᵀ·x, dWd = dyᵀ·h, those whose pointer is set,
+ *                in dtype, or in fp32 with w_grad_f32
+ * Inputs and the stride ld_f of h, a, b, dg, du: 16-byte aligned, strides multiples
+ * of 8.  y, dx and the weight gradients are dense, of any alignment.         */
+enum { DSALT_ACT_SILU = 0, DSALT_ACT_GELU = 1, DSALT_ACT_GELU_TANH = 2 };
+typedef struct DsaltGatedFfnParams {
+  const void* x;              /* [T, d] stride ld_x */
+  const void* w_gate;         /* [F, d] stride ld_wg */
+  const void* w_up;           /* [F, d] stride ld_wu */
+  const void* w_down;         /* [d_out, F] stride ld_wd */
+  void* h;                    /* [T, F] stride ld_f */
+  void* a;                    /* [T, F] stride ld_f, or NULL (inference) */
+  void* b;                    /* [T, F] stride ld_f, or NULL */
+  void* y;                    /* [T, d_out] */
+  const void* dy;             /* [T, d_out] stride ld_dy        (backward) */
+  void* dg;                   /* [T, F] stride ld_f */
+  void* du;                   /* [T, F] stride ld_f */
+  void* dx;                   /* [T, d] */
+  void* dw_gate;              /* [F, d], or NULL */
+  void* dw_up;                /* [F, d], or NULL */
+  void* dw_down;              /* [d_out, F], or NULL */
+  int32_t* status;            /* device status word, or NULL */
+  int64_t T;
+  int64_t ld_x, ld_wg, ld_wu, ld_wd, ld_f, ld_dy;
+  int32_t d, F, d_out;
+  int32_t activation;
+  int32_t dtype;
+  int32_t w_grad_f32;
+} DsaltGatedFfnParams;
+DSALT_API int dsalt_gated_ffn_hidden(const DsaltGatedFfnParams* p, void* stream);
+DSALT_API int dsalt_gated_ffn_out(const DsaltGatedFfnParams* p, void* stream);
+DSALT_API int dsalt_gated_ffn_bwd_hidden(const DsaltGatedFfnParams* p, void* stream);
+DSALT_API int dsalt_gated_ffn_bwd_input(const DsaltGatedFfnParams* p, void* stream);
+DSALT_API int dsalt_gated_ffn_bwd_weights(const DsaltGatedFfnParams* p, void* stream);
+
+/* Dropout without a stored mask, f16 / bf16 / f32.  Element i (row-major index) is
+ * dropped when its 16-bit draw is below `threshold` = round(p·65536); kept elements
+ * are multiplied by 65536 / (65536 − threshold).  The draws: Philox4x32-10 (Salmon,
+ * Moraes, Dror, Shaw, SC 2011) with key = *seed (low word, high word) and counter
+ * (i / 8 low, i / 8 high, site, 0); draw i % 8 is a half of output word (i % 8) / 2,
+ * the low half first.  A backward is the same call on the gradient.         */
+typedef struct DsaltDropoutParams {
+  const void* x;              /* [n] dtype */
+  void* y;                    /* [n] dtype; may be x */
+  const int64_t* seed;        /* device scalar, read by the kernel */
+  int64_t n;
+  uint32_t site;
+  int32_t threshold;          /* 0 … 65536 */
+  int32_t dtype;
+} DsaltDropoutParams;
+DSALT_API int dsalt_dropout(const DsaltDropoutParams* p, void* stream);
+
+/* Between a block and the next: the norm of the block's output f, its gate and
+ * residual scale, dropout, the residual add and the norm before the next block.
+ *   n  = f·rf·post,  rf = 1/sqrt(mean(f²) + eps)         (n = f without post)
+ *   x' = R(x + D(scale⊙gate⊙n)),  D as dsalt_dropout on [T, d]
+ *   h  = R(x'·r·norm), r = 1/sqrt(mean(x'²) + eps)       (with norm set)
+ * and the backward, from the gradients of x' (dx_new) and h (dh), either NULL for 0:
+ *   G  = dx_new + r·(dh⊙norm − x'·r²·mean(dh⊙norm⊙x')),  dx = R(G),
+ *   dn = D(G)⊙scale⊙gate,  df = R(rf·(dn⊙post − f·rf²·mean(dn⊙post⊙f))),
+ *   dgate = D(G)⊙scale⊙n (summed over the columns for a gate per token),
+ *   dscale = Σ_t D(G)⊙gate⊙n,  dpost = Σ_t dn⊙f·rf,  dnorm = Σ_t dh⊙x'·r,
+ * all in fp32 with one rounding each; the Σ_t in a fixed order through `parts`
+ * (dsalt_residual_norm_parts(T, d) rows of 3·d fp32).  f16 / bf16 / f32, any d up to
+ * DSALT_RESIDUAL_MAX_D; dense rows.                                          */
+#define DSALT_RESIDUAL_MAX_D 16384
+enum { DSALT_GATE_NONE = 0, DSALT_GATE_TOKEN = 1, DSALT_GATE_FULL = 2 };
+typedef struct DsaltResidualNormParams {
+  const void* x;              /* [T, d]                          (forward) */
+  const void* f;              /* [T, d] */
+  const void* gate;           /* [T] or [T, d] dtype, by gate_mode */
+  const void* post;           /* [d] weights: fp32 with w_f32, else dtype; NULL: none */
+  const void* scale;          /* [d], or NULL */
+  const void* norm;           /* [d], or NULL (no h) */
+  void* x_new;                /* [T, d] written by the forward, read by the backward */
+  void* h;                    /* [T, d]                          (forward) */
+  float* rf;                  /* [T]: written by the forward when set, read by the backward (with post) */
+  float* r;                   /* [T]: likewise (with norm) */
+  const void* dx_new;         /* [T, d], or NULL                (backward) */
+  const void* dh;             /* [T, d], or NULL */
+  void* dx;                   /* [T, d] */
+  void* df;                   /* [T, d] */
+  void* dgate;                /* like gate */
+  void* dpost;                /* [d] like the weights, or NULL */
+  void* dscale;               /* [d], or NULL */
+  void* dnorm;                /* [d], or NULL */
+  float* parts;               /* backward scratch */
+  const int64_t* seed;        /* device scalar; needed when threshold > 0 */
+  int64_t T;
+  int32_t d;
+  float eps;
+  uint32_t site;
+  int32_t threshold;
+  int32_t gate_mode;
+  int32_t dtype;
+  int32_t w_f32;
+} DsaltResidualNormParams;
+DSALT_API int dsalt_residual_norm_fwd(const DsaltResidualNormParams* p, void* stream);
+DSALT_API int dsalt_residual_norm_bwd(const DsaltResidualNormParams* p, void* stream);
+/* partial rows of the backward's scratch on the current device; negative: a status code negated */
+DSALT_API int dsalt_residual_norm_parts(int64_t T, int32_t d);
+
 /* ---- self-test of the failure path ---------------------------------------
  * Launches one CTA whose mbarrier wait can never complete.  The bounded wait
  * every tensor-core kernel uses gives up after its limit (about 2 s), ORs
@@ -504,7 +615,7 @@ DSALT_API const char* dsalt_b200_status_string(int status);
 /* sizeof of the parameter structs, for bindings to check their mirrors:
  * which = 0 schedule, 1 gather, 2 attn, 3 score, 4 topk, 5 win_gate, 6 rope,
  * 7 rmsnorm, 8 scale_rows, 9 xent, 10 swiglu, 11 win_gate_bwd,
- * 12 score_bwd                                                              */
+ * 12 score_bwd, 13 gqa_reduce, 14 gated_ffn, 15 dropout, 16 residual_norm     */
 DSALT_API int dsalt_b200_params_sizeof(int which);
 
 #ifdef __cplusplus
