@@ -4,12 +4,10 @@
 #include <mutex>
 
 #include "ffn.cuh"
-#include "sm100.cuh"
+#include "tc_pair.cuh"
 
 namespace dsalt {
-CUresult encode_tensor_map_3d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t d0, uint64_t d1,
-                              uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0,
-                              uint32_t box1, uint32_t box2) {
+static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -19,6 +17,13 @@ CUresult encode_tensor_map_3d(CUtensorMap* m, CUtensorMapDataType dt, const void
         q == cudaDriverEntryPointSuccess)
       fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
   });
+  return fn;
+}
+
+CUresult encode_tensor_map_3d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t d0, uint64_t d1,
+                              uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0,
+                              uint32_t box1, uint32_t box2) {
+  const PFN_cuTensorMapEncodeTiled_v12000 fn = tensor_map_encoder();
   if (!fn) return CUDA_ERROR_NOT_FOUND;
   cuuint64_t dims[3] = {d0, d1, d2};
   cuuint64_t strides[2] = {stride1_bytes, stride2_bytes};
@@ -26,6 +31,20 @@ CUresult encode_tensor_map_3d(CUtensorMap* m, CUtensorMapDataType dt, const void
   cuuint32_t es[3] = {1, 1, 1};
   return fn(m, dt, 3, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+// As a 3-D map with one plane, so that the 3-D loads and stores serve it.
+CUresult encode_tensor_map_2d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t rows, uint64_t cols,
+                              uint64_t stride_bytes, uint32_t box_cols, uint32_t box_rows, int swizzle_bytes) {
+  const PFN_cuTensorMapEncodeTiled_v12000 fn = tensor_map_encoder();
+  if (!fn) return CUDA_ERROR_NOT_FOUND;
+  cuuint64_t dims[3] = {cols, rows, 1};
+  cuuint64_t strides[2] = {stride_bytes, stride_bytes};
+  cuuint32_t box[3] = {box_cols, box_rows, 1};
+  cuuint32_t es[3] = {1, 1, 1};
+  return fn(m, dt, 3, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 }  // namespace dsalt
 
@@ -410,17 +429,17 @@ static int check_ffn(const DsaltGatedFfnParams* p, int stage) {
   struct In { const void* ptr; int64_t ld, width; };
   const In x = {p->x, p->ld_x, p->d}, wg = {p->w_gate, p->ld_wg, p->d}, wu = {p->w_up, p->ld_wu, p->d},
            wd = {p->w_down, p->ld_wd, p->F}, dy = {p->dy, p->ld_dy, p->d_out}, h = {p->h, p->ld_f, p->F},
-           a = {p->a, p->ld_f, p->F}, b = {p->b, p->ld_f, p->F}, dg = {p->dg, p->ld_f, p->F}, du = {p->du, p->ld_f, p->F};
-  In need[6];
+           a = {p->a, p->ld_f, p->F}, b = {p->b, p->ld_f, p->F}, ab = {p->ab, p->ld_f, p->F}, dg = {p->dg, p->ld_f, p->F}, du = {p->du, p->ld_f, p->F};
+  In need[8];
   int n = 0;
   switch (stage) {
     case FFN_HIDDEN:
-      if ((p->a == nullptr) != (p->b == nullptr)) return DSALT_ERR_ARG;
+      if ((p->a == nullptr) != (p->b == nullptr) || (p->a == nullptr) != (p->ab == nullptr)) return DSALT_ERR_ARG;
       need[n++] = x; need[n++] = wg; need[n++] = wu; need[n++] = h;
-      if (p->a) { need[n++] = a; need[n++] = b; }
+      if (p->a) { need[n++] = a; need[n++] = b; need[n++] = ab; }
       break;
     case FFN_OUT: need[n++] = h; need[n++] = wd; break;
-    case FFN_BWD_HIDDEN: need[n++] = dy; need[n++] = wd; need[n++] = a; need[n++] = b; need[n++] = dg; need[n++] = du; break;
+    case FFN_BWD_HIDDEN: need[n++] = dy; need[n++] = wd; need[n++] = a; need[n++] = b; need[n++] = ab; need[n++] = dg; need[n++] = du; break;
     case FFN_BWD_INPUT: need[n++] = dg; need[n++] = du; need[n++] = wg; need[n++] = wu; break;
     default:
       if (p->dw_gate) need[n++] = dg;

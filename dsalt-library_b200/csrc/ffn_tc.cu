@@ -17,43 +17,51 @@
 // Bound: the tensor pipe for long batches (6·T·d·F flops forward, 12·T·d·F
 // backward), the weights' bytes for few tokens.
 //
-// A tile is 128 tokens × 256 columns, K in steps of 64 through a TMA ring; the
-// accumulators are double-buffered in TMEM (2 × 256 columns), so that a tile's
-// epilogue runs beside the next tile's products.
-//   warp 0      TMA loads (128-byte swizzle)
-//   warp 1      TMEM owner, single-thread MMA issuer
-//   warps 2-9   epilogue: TMEM lane quadrant warp % 4, column half (warp − 2) / 4
+// A tile is 256 rows × BN columns worked on by a pair of CTAs (a cluster of 2,
+// cta_group::2): each holds 128 rows of A, half of B's columns and the accumulator of
+// its rows, so that an SM fetches two thirds of what a tile of its own would need.
+// K in steps of 64 through a TMA ring; two accumulators in TMEM (2 × BN columns), so
+// that a tile's epilogue runs beside the next tile's products.
+//   warp 0      TMA loads of this CTA's halves (128-byte swizzle); the leader's FULL
+//               barrier counts both CTAs' bytes
+//   warp 1      TMEM owner; in the leader the single-thread MMA issuer
+//   warps 2-17  epilogue: TMEM lane quadrant warp % 4, every fourth 32-column chunk;
+//               results go through 64-byte-swizzled staging and TMA stores
 // Every wait is bounded (sm100::mbar_wait).
 #include <algorithm>
 #include <cstring>
 
 #include "ffn.cuh"
-#include "sm100.cuh"
+#include "tc_pair.cuh"
 
 namespace dsalt {
 namespace ffn {
 
-constexpr int BM = 128, BN = 256, BK = 64;
+constexpr int BM = 256, BK = 64;
 constexpr int kPiece = 128 * BK * 2;       // 128 rows (or columns) × 64 K of one operand
-constexpr int kStageBytes = 3 * kPiece;    // A, and B's two halves
-constexpr int kStages = 4;
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 16;
 constexpr int kThreads = (2 + kEpiWarps) * 32;
-constexpr int kWarpStage = 4096;           // epilogue staging of one warp
+constexpr int kBox = 2048;                 // staged box: 32 rows × 64 bytes
 constexpr int kMaxProb = 3;
-enum { FULL = 0, EMPTY = FULL + kStages, ACC_FULL = EMPTY + kStages, ACC_EMPTY = ACC_FULL + 2, FINAL = ACC_EMPTY + 2,
-       NB = FINAL + 1 };
 enum Epi { EPI_STORE = 0, EPI_HIDDEN = 1, EPI_DHIDDEN = 2 };
 
-struct alignas(1024) Smem {
-  uint8_t ring[kStages][kStageBytes];
-  uint8_t stage[kEpiWarps][kWarpStage];
-  uint64_t bars[NB];
-  uint32_t tmem_base;
-  int abort_flag;
+template <int BN, int EPI>
+struct Cfg {
+  static constexpr int kStageBytes = kPiece + BN / 2 * BK * 2;  // A's and B's halves of this CTA
+  static constexpr int kBoxes = EPI == EPI_DHIDDEN ? 3 : 2;     // staged boxes of a warp
+  static constexpr int kStages = BN == 256 ? (EPI == EPI_DHIDDEN ? 4 : 5) : 6;
+  static constexpr int FULL = 0, EMPTY = kStages, ACC_FULL = 2 * kStages, ACC_EMPTY = ACC_FULL + 2,
+                       FINAL = ACC_EMPTY + 2, LOADED = FINAL + 1, NB = LOADED + kEpiWarps;
+  struct alignas(1024) Smem {
+    uint8_t ring[kStages][kStageBytes];
+    uint8_t stage[kEpiWarps][kBoxes * kBox];
+    uint64_t bars[NB];
+    uint32_t tmem_base;
+    int abort_flag;
+  };
 };
 
-// One product D[M, N] = Σ over its K segments; out_cols: columns of D.
+// One product D[M, N] = Σ over its K segments.
 struct Problem {
   int M, N, m_tiles, n_tiles, tile_end;
   void* out;
@@ -62,13 +70,10 @@ struct Problem {
 
 struct alignas(64) Args {
   CUtensorMap ma[kMaxProb], mb[kMaxProb];  // per problem, or per K segment of the only problem
+  CUtensorMap mo[5];                       // store: out of each problem; hidden: h, a, b, ab; dhidden: a, b, ab, du, dg
   Problem prob[kMaxProb];
   int n_prob, n_seg, K, n_tiles;
-  bool bf16, out_f32;
-  int act;
-  void *h, *a, *b;        // hidden: outputs (a, b may be null); dhidden: a, b inputs
-  void *dg, *du;          // dhidden outputs
-  int64_t ld_f;
+  bool bf16, out_f32, out_tma, keep;
   int32_t* status;
 };
 
@@ -87,21 +92,23 @@ __device__ __forceinline__ Tile decode(const Args& a, int t) {
 // ---------------------------------------------------------------- activation
 // act(g) and act'(g).  exp and the reciprocal are the fast ones (relative error
 // below 2^-20 over the range where the result is not rounded to 0 or g): the
-// results are rounded to 16 bits next.
-__device__ __forceinline__ void act_pair(int act, float g, float& a, float& da) {
-  if (act == DSALT_ACT_SILU) {
-    const float sig = __fdividef(1.f, 1.f + __expf(-g));
+// results are rounded to 16 or 24 bits next.
+template <int ACT>
+__device__ __forceinline__ void act_pair(float g, float& a, float& da) {
+  constexpr float kLog2e = 1.4426950409f;
+  if constexpr (ACT == DSALT_ACT_SILU) {
+    const float sig = sm100::fast_rcp(1.f + sm100::fast_exp2(-kLog2e * g));
     a = g * sig;
-    da = sig * (1.f + g - a);
-  } else if (act == DSALT_ACT_GELU) {
+    da = fmaf(a, 1.f - sig, sig);
+  } else if constexpr (ACT == DSALT_ACT_GELU) {
     const float cdf = normcdff(g);
     a = g * cdf;
-    da = fmaf(g * 0.3989422804f, __expf(-0.5f * g * g), cdf);
+    da = fmaf(g * 0.3989422804f, sm100::fast_exp2(-0.5f * kLog2e * g * g), cdf);
   } else {
     // ½(1 + tanh z) = σ(2z), ½(1 − tanh² z) = 2σ(1 − σ), z = √(2/π)(g + 0.044715 g³)
     const float g2 = g * g;
     const float z2 = 1.5957691216f * g * fmaf(0.044715f, g2, 1.f);
-    const float sig = __fdividef(1.f, 1.f + __expf(-z2));
+    const float sig = sm100::fast_rcp(1.f + sm100::fast_exp2(-kLog2e * z2));
     const float w = sig * (1.f - sig);
     a = g * sig;
     da = sig + (w > 0.f ? g * w * 1.5957691216f * fmaf(0.134145f, g2, 1.f) : 0.f);
@@ -109,154 +116,134 @@ __device__ __forceinline__ void act_pair(int act, float g, float& a, float& da) 
 }
 
 // ------------------------------------------------------------------- staging
-// A warp's 32 rows × ROWB bytes, in 16-byte units XORed so that a row's owner
-// and a row-contiguous copy both touch all banks.
-template <int ROWB>
-__device__ __forceinline__ uint32_t stage_off(int row, int u) {
-  if constexpr (ROWB == 128) return row * 128 + ((u ^ (row & 7)) << 4);
-  return row * 64 + ((u ^ ((row >> 1) & 3)) << 4);
+// A box of 32 rows × 64 bytes in TMA's 64-byte swizzle (16-byte units XORed with
+// row / 2 % 4): a row's owner writes its four units without bank conflicts.
+__device__ __forceinline__ uint32_t box_off(int row, int u) { return row * 64 + ((u ^ ((row >> 1) & 3)) << 4); }
+
+// this lane's row of 32 values, rounded to 16 bits
+__device__ __forceinline__ void stage_row16(uint8_t* box, int lane, const float* v, bool bf16) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    *reinterpret_cast<uint4*>(box + box_off(lane, u)) =
+        make_uint4(sm100::pack2(v[8 * u + 0], v[8 * u + 1], bf16), sm100::pack2(v[8 * u + 2], v[8 * u + 3], bf16),
+                   sm100::pack2(v[8 * u + 4], v[8 * u + 5], bf16), sm100::pack2(v[8 * u + 6], v[8 * u + 7], bf16));
 }
-// staged rows → global rows r0 … (at most `rows`), columns c0 … below N
-template <int ROWB, typename E>
-__device__ __forceinline__ void stage_to_global(const uint8_t* st, E* out, int64_t ld, int rows, int c0, int N, bool vec) {
-  constexpr int kU = ROWB / 16, kE = 16 / sizeof(E);
+__device__ __forceinline__ void stage_words(uint8_t* box, int lane, const uint32_t* w) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    *reinterpret_cast<uint4*>(box + box_off(lane, u)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+}
+// a staged box → global rows and columns inside [rows, N), element by element: results
+// whose rows are not 16-byte aligned (no tensor map describes them)
+template <typename E>
+__device__ __forceinline__ void box_to_global(const uint8_t* box, E* out, int64_t ld, int rows, int c0, int N) {
+  constexpr int kCols = 64 / sizeof(E);
   const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < kU; ++i) {
-    const int idx = i * 32 + lane, row = idx / kU, u = idx % kU;
-    const int c = c0 + u * kE;
-    if (row >= rows || c >= N) continue;
-    const uint4 v = *reinterpret_cast<const uint4*>(st + stage_off<ROWB>(row, u));
-    E* dst = out + row * ld + c;
-    if (vec && c + kE <= N) {
-      *reinterpret_cast<uint4*>(dst) = v;
-    } else {
-      const E* e = reinterpret_cast<const E*>(&v);
-      for (int k = 0; k < kE && c + k < N; ++k) dst[k] = e[k];
-    }
+  for (int i = lane; i < 32 * kCols; i += 32) {
+    const int row = i / kCols, c = i % kCols;
+    if (row < rows && c0 + c < N)
+      out[row * ld + c0 + c] = *reinterpret_cast<const E*>(box + box_off(row, c * (int)sizeof(E) / 16) + c * sizeof(E) % 16);
   }
 }
-// global rows → staging (units past the bounds as zeros); 16-byte aligned rows
-template <int ROWB>
-__device__ __forceinline__ void global_to_stage(uint8_t* st, const uint16_t* in, int64_t ld, int rows, int c0, int N) {
-  constexpr int kU = ROWB / 16;
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < kU; ++i) {
-    const int idx = i * 32 + lane, row = idx / kU, u = idx % kU;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row < rows && c0 + u * 8 < N) v = *reinterpret_cast<const uint4*>(in + row * ld + c0 + u * 8);
-    *reinterpret_cast<uint4*>(st + stage_off<ROWB>(row, u)) = v;
-  }
-}
-// this lane's row of 32 values → 4 units of the staged 16-bit rows
-__device__ __forceinline__ void stage_row16(uint8_t* st, int lane, const float* v, bool bf16) {
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    uint4 w;
-    w.x = sm100::pack2(v[8 * u + 0], v[8 * u + 1], bf16);
-    w.y = sm100::pack2(v[8 * u + 2], v[8 * u + 3], bf16);
-    w.z = sm100::pack2(v[8 * u + 4], v[8 * u + 5], bf16);
-    w.w = sm100::pack2(v[8 * u + 6], v[8 * u + 7], bf16);
-    *reinterpret_cast<uint4*>(st + stage_off<64>(lane, u)) = w;
-  }
-}
-__device__ __forceinline__ float2 unpack2(uint32_t w, bool bf16) {
-  if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+// bytes 2 and 3 of two words: the upper 16 bits of fp32 x (low half) and y
+__device__ __forceinline__ uint32_t upper16(float x, float y) {
+  return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
 }
 
 // ------------------------------------------------------------------- kernel
 // AMN / BMN: the operand's K is the strided dimension (MN-major) instead of the
-// contiguous one.  A 128-wide piece of an operand at K offset k0:
-//   K-major   one box of 64 k × 128 rows; MMA step k at +32·k bytes
-//   MN-major  two boxes of 64 columns × 64 k; MMA step k at +2048·k bytes
-template <bool MN>
+// contiguous one.  A piece of W rows (or columns) of an operand at K offset k0:
+//   K-major   one box of 64 k × W rows; MMA step k at +32·k bytes
+//   MN-major  W / 64 boxes of 64 columns × 64 k; MMA step k at +2048·k bytes
+template <bool MN, int W>
 __device__ __forceinline__ void load_piece(uint32_t dst, const CUtensorMap* map, uint32_t bar, int mn0, int k0) {
   if constexpr (MN) {
-    sm100::tma_load_3d(dst, map, bar, mn0, k0, 0);
-    sm100::tma_load_3d(dst + kPiece / 2, map, bar, mn0 + 64, k0, 0);
+#pragma unroll
+    for (int c = 0; c < W; c += 64) sm100::tma_load_3d_pair(dst + c * 128, map, bar, mn0 + c, k0, 0);
   } else {
-    sm100::tma_load_3d(dst, map, bar, k0, mn0, 0);
+    sm100::tma_load_3d_pair(dst, map, bar, k0, mn0, 0);
   }
 }
 template <bool MN>
 __device__ __forceinline__ uint64_t piece_desc(uint32_t addr, int kk) {
-  return MN ? sm100::sdesc_sw128(addr + kk * 2048, kPiece / 2, 1024) : sm100::sdesc_sw128(addr + kk * 32, 16, 1024);
+  return MN ? sm100::sdesc_sw128(addr + kk * 2048, 64 * 128, 1024) : sm100::sdesc_sw128(addr + kk * 32, 16, 1024);
 }
 
-template <bool AMN, bool BMN, int EPI>
-__global__ void __launch_bounds__(kThreads, 1) ffn_gemm_kernel(const __grid_constant__ Args a) {
+template <bool AMN, bool BMN, int EPI, int BN, int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) ffn_gemm_kernel(const __grid_constant__ Args a) {
   using namespace sm100;
+  using C = Cfg<BN, EPI>;
+  constexpr int kStages = C::kStages;
   extern __shared__ uint8_t smem_raw[];
-  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  auto& sm = *reinterpret_cast<typename C::Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_rank();
   const BarArray bar{smem_u32(&sm.bars[0])};
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(bar[FULL + s], 1);
-      mbar_init(bar[EMPTY + s], 1);
+      mbar_init(bar[C::FULL + s], 1);
+      mbar_init(bar[C::EMPTY + s], 1);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(bar[ACC_FULL + b], 1);
-      mbar_init(bar[ACC_EMPTY + b], kEpiWarps);
+      mbar_init(bar[C::ACC_FULL + b], 1);
+      mbar_init(bar[C::ACC_EMPTY + b], 2 * kEpiWarps);
     }
-    mbar_init(bar[FINAL], 1);
+    mbar_init(bar[C::FINAL], 1);
+    for (int w = 0; w < kEpiWarps; ++w) mbar_init(bar[C::LOADED + w], 1);
     fence_mbar_init();
     sm.abort_flag = 0;
   }
-  if (warp == 1) tmem_alloc(smem_u32(&sm.tmem_base), 512);
+  if (warp == 1) tmem_alloc_pair(smem_u32(&sm.tmem_base), 2 * BN);
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // both CTAs' barriers exist before either signals the other's
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
   volatile int* abort_flag = &sm.abort_flag;
   const int k_tiles = (a.K + BK - 1) / BK;
   const int steps = k_tiles * a.n_seg;
+  const int t0 = blockIdx.x >> 1, t_step = gridDim.x >> 1;
 
   if (warp == 0) {
     // ------------------------------------------------------------ loads
     if (lane == 0) {
       int g = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < a.n_tiles; t += gridDim.x) {
+      for (int t = t0; ok && t < a.n_tiles; t += t_step) {
         const Tile tl = decode(a, t);
-        for (int s = 0; ok && s < steps; ++s, ++g) {
+        for (int s = 0; s < steps; ++s, ++g) {
           const int st = g % kStages;
-          if (g >= kStages && !mbar_wait(bar[EMPTY + st], (g / kStages - 1) & 1, abort_flag, a.status)) {
+          if (g >= kStages && !mbar_wait(bar[C::EMPTY + st], (g / kStages - 1) & 1, abort_flag, a.status)) {
             ok = false;
             break;
           }
           const int seg = s / k_tiles, k0 = (s - seg * k_tiles) * BK;
           const int im = a.n_prob > 1 ? tl.prob : seg;
-          const uint32_t base = smem_u32(sm.ring[st]);
-          mbar_expect_tx(bar[FULL + st], kStageBytes);
-          load_piece<AMN>(base, &a.ma[im], bar[FULL + st], tl.m0, k0);
-          if constexpr (EPI == EPI_HIDDEN) {  // the same 128 columns of gate and up
-            load_piece<BMN>(base + kPiece, &a.mb[0], bar[FULL + st], tl.nt * 128, k0);
-            load_piece<BMN>(base + 2 * kPiece, &a.mb[1], bar[FULL + st], tl.nt * 128, k0);
-          } else {
-            load_piece<BMN>(base + kPiece, &a.mb[im], bar[FULL + st], tl.nt * BN, k0);
-            load_piece<BMN>(base + 2 * kPiece, &a.mb[im], bar[FULL + st], tl.nt * BN + 128, k0);
-          }
+          const uint32_t base = smem_u32(sm.ring[st]), full = map_rank(bar[C::FULL + st], 0);
+          if (rank == 0) mbar_expect_tx(bar[C::FULL + st], 2 * C::kStageBytes);
+          load_piece<AMN, 128>(base, &a.ma[im], full, tl.m0 + 128 * rank, k0);
+          if constexpr (EPI == EPI_HIDDEN)  // the same columns of gate (leader) and up (its peer)
+            load_piece<BMN, BN / 2>(base + kPiece, &a.mb[rank], full, tl.nt * (BN / 2), k0);
+          else
+            load_piece<BMN, BN / 2>(base + kPiece, &a.mb[im], full, tl.nt * BN + (BN / 2) * rank, k0);
         }
       }
-      // never leave a copy in flight into shared memory
-      for (int gg = max(0, g - kStages); gg < g; ++gg) mbar_drain(bar[FULL + gg % kStages], (gg / kStages) & 1);
+      // the last products have read this CTA's shared memory, and their signals have come
+      for (int gg = max(0, g - kStages); gg < g; ++gg) mbar_drain(bar[C::EMPTY + gg % kStages], (gg / kStages) & 1);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       const uint32_t idesc = idesc_f16(a.bf16, BM, BN, AMN, BMN);
       int g = 0, li = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < a.n_tiles; t += gridDim.x, ++li) {
+      for (int t = t0; ok && t < a.n_tiles; t += t_step, ++li) {
         const int acc = li & 1;
-        if (li >= 2) ok = mbar_wait(bar[ACC_EMPTY + acc], ((li >> 1) - 1) & 1, abort_flag, a.status);
+        if (li >= 2) ok = mbar_wait(bar[C::ACC_EMPTY + acc], ((li >> 1) - 1) & 1, abort_flag, a.status);
         tc_fence_after();
         for (int s = 0; ok && s < steps; ++s, ++g) {
           const int st = g % kStages;
-          if (!mbar_wait(bar[FULL + st], (g / kStages) & 1, abort_flag, a.status)) {
+          if (!mbar_wait(bar[C::FULL + st], (g / kStages) & 1, abort_flag, a.status)) {
             ok = false;
             break;
           }
@@ -264,135 +251,195 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_gemm_kernel(const __grid_cons
           const uint32_t base = smem_u32(sm.ring[st]);
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk)
-            mma_f16(tmem + acc * BN, piece_desc<AMN>(base, kk), piece_desc<BMN>(base + kPiece, kk), idesc,
-                    (s > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(bar[EMPTY + st]);
+            mma_f16_pair(tmem + acc * BN, piece_desc<AMN>(base, kk), piece_desc<BMN>(base + kPiece, kk), idesc,
+                         (s > 0 || kk > 0) ? 1u : 0u);
+          mma_commit_pair(bar[C::EMPTY + st]);
         }
-        if (ok) mma_commit(bar[ACC_FULL + acc]);
+        if (ok) mma_commit_pair(bar[C::ACC_FULL + acc]);
       }
-      mma_commit(bar[FINAL]);
-      mbar_drain(bar[FINAL], 0);
+      mma_commit_pair(bar[C::FINAL]);
     }
+    if (lane == 0) mbar_drain(bar[C::FINAL], 0);
   } else {
     // ------------------------------------------------------------ epilogue
-    const int q4 = warp & 3, half = (warp - 2) >> 2;
+    const int q4 = warp & 3, cg = (warp - 2) >> 2;
     const uint32_t lane_addr = (uint32_t)(32 * q4) << 16;
-    uint8_t* st0 = sm.stage[warp - 2];
-    int li = 0;
-    for (int t = blockIdx.x; t < a.n_tiles; t += gridDim.x, ++li) {
+    uint8_t* box = sm.stage[warp - 2];
+    const uint32_t box_u32 = smem_u32(box);
+    int li = 0, loads = 0;
+    // a box that this warp staged → its place in global memory
+    auto store_box = [&](const CUtensorMap* map, int i, int col, int row) {
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(map, box_u32 + i * kBox, col, row, 0);
+        bulk_commit();
+      }
+    };
+    for (int t = t0; t < a.n_tiles; t += t_step, ++li) {
       const Tile tl = decode(a, t);
       const Problem& pr = a.prob[tl.prob];
       const int acc = li & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(bar[ACC_FULL + acc], (li >> 1) & 1, abort_flag, a.status))) break;
+      const int row0 = tl.m0 + 128 * (int)rank + 32 * q4, rows = pr.M - row0;  // rows of this warp (may be <= 0)
+      constexpr int kCols = EPI == EPI_HIDDEN ? BN / 2 : BN;                   // result columns of a tile
+      const int col0 = tl.nt * kCols;
+      auto load_ab = [&](int c) {  // the a, b and ab boxes of columns c (dhidden)
+        if (lane == 0) {
+          bulk_wait_read<0>();  // the boxes' last results are out
+          mbar_expect_tx(bar[C::LOADED + warp - 2], 3 * kBox);
+#pragma unroll
+          for (int i = 0; i < 3; ++i)
+            tma_load_3d(box_u32 + i * kBox, &a.mo[i], bar[C::LOADED + warp - 2], col0 + c, row0, 0);
+        }
+      };
+      if constexpr (EPI == EPI_DHIDDEN)
+        if (cg * 32 < kCols) load_ab(cg * 32);
+      const bool full = mbar_wait(bar[C::ACC_FULL + acc], (li >> 1) & 1, abort_flag, a.status);
+      if (!__all_sync(0xffffffffu, full)) {
+        if (EPI == EPI_DHIDDEN && cg * 32 < kCols && lane == 0) mbar_drain(bar[C::LOADED + warp - 2], loads & 1);
+        break;
+      }
       tc_fence_after();
       const uint32_t tacc = tmem + acc * BN + lane_addr;
-      const int row0 = tl.m0 + 32 * q4, rows = pr.M - row0;  // rows of this warp (may be <= 0)
-      if constexpr (EPI == EPI_HIDDEN) {
+      bool lost = false;
 #pragma unroll 1
-        for (int c = half * 64; c < half * 64 + 64; c += 32) {
-          float g[32], u[32];
-          tmem_ld32(tacc + c, g);
-          tmem_ld32(tacc + 128 + c, u);
-          tmem_wait_ld();
-          const int col = tl.nt * 128 + c;
-          const int64_t at = (int64_t)row0 * a.ld_f;
-          float b[32];
+      for (int c = cg * 32; c < kCols; c += 128) {
+        if constexpr (EPI == EPI_HIDDEN) {
+          uint32_t wh[16], wa[16], wb[16], wl[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            float av, da;
-            act_pair(a.act, g[j], av, da);
-            g[j] = av;
-            b[j] = u[j] * da;
-            u[j] *= av;
+          for (int c2 = 0; c2 < 32; c2 += 16) {  // 16 columns at a time: the values fit the registers
+            float g[16], u[16];
+            tmem_ld16(tacc + c + c2, g);
+            tmem_ld16(tacc + BN / 2 + c + c2, u);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+              float a0, a1, d0, d1;
+              act_pair<ACT>(g[j], a0, d0);
+              act_pair<ACT>(g[j + 1], a1, d1);
+              d0 *= u[j];
+              d1 *= u[j + 1];
+              const int k = (c2 + j) / 2;
+              wh[k] = pack2(u[j] * a0, u[j + 1] * a1, a.bf16);
+              wa[k] = upper16(a0, a1);
+              wb[k] = upper16(d0, d1);
+              // byte 1 of a0, d0, a1, d1
+              wl[k] = __byte_perm(__byte_perm(__float_as_uint(a0), __float_as_uint(d0), 0x0051),
+                                  __byte_perm(__float_as_uint(a1), __float_as_uint(d1), 0x0051), 0x5410);
+            }
           }
-          stage_row16(st0, lane, u, a.bf16);
-          stage_row16(st0 + 2048, lane, g, a.bf16);
+          if (lane == 0) bulk_wait_read<0>();
           __syncwarp();
-          stage_to_global<64>(st0, (uint16_t*)a.h + at, a.ld_f, rows, col, pr.N, true);
-          if (a.a) {
-            stage_to_global<64>(st0 + 2048, (uint16_t*)a.a + at, a.ld_f, rows, col, pr.N, true);
+          stage_words(box, lane, wh);
+          store_box(&a.mo[0], 0, col0 + c, row0);
+          if (a.keep) {
+            stage_words(box + kBox, lane, wa);
+            store_box(&a.mo[1], 1, col0 + c, row0);
+            if (lane == 0) bulk_wait_read<1>();
             __syncwarp();
-            stage_row16(st0, lane, b, a.bf16);
+            stage_words(box, lane, wb);
+            store_box(&a.mo[2], 0, col0 + c, row0);
+            if (lane == 0) bulk_wait_read<1>();
             __syncwarp();
-            stage_to_global<64>(st0, (uint16_t*)a.b + at, a.ld_f, rows, col, pr.N, true);
+            stage_words(box + kBox, lane, wl);
+            store_box(&a.mo[3], 1, col0 + c, row0);
           }
-          __syncwarp();
-        }
-      } else if constexpr (EPI == EPI_DHIDDEN) {
-#pragma unroll 1
-        for (int c = half * 128; c < half * 128 + 128; c += 32) {
-          const int col = tl.nt * BN + c;
-          const int64_t at = (int64_t)row0 * a.ld_f;
-          global_to_stage<64>(st0, (const uint16_t*)a.a + at, a.ld_f, rows, col, pr.N);
-          global_to_stage<64>(st0 + 2048, (const uint16_t*)a.b + at, a.ld_f, rows, col, pr.N);
+        } else if constexpr (EPI == EPI_DHIDDEN) {
           float v[32];
           tmem_ld32(tacc + c, v);
           tmem_wait_ld();
-          __syncwarp();
+          if (!__all_sync(0xffffffffu, mbar_wait(bar[C::LOADED + warp - 2], loads & 1, abort_flag, a.status))) {
+            lost = true;
+            break;
+          }
+          ++loads;
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            uint4* pa = reinterpret_cast<uint4*>(st0 + stage_off<64>(lane, u));
-            uint4* pb = reinterpret_cast<uint4*>(st0 + 2048 + stage_off<64>(lane, u));
-            uint32_t wa[4], wb[4];
-            *reinterpret_cast<uint4*>(wa) = *pa;
-            *reinterpret_cast<uint4*>(wb) = *pb;
+            uint4* pa = reinterpret_cast<uint4*>(box + box_off(lane, u));
+            uint4* pb = reinterpret_cast<uint4*>(box + kBox + box_off(lane, u));
+            const uint4 va = *pa, vb = *pb, vl = *reinterpret_cast<const uint4*>(box + 2 * kBox + box_off(lane, u));
+            uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
+            const uint32_t wl[4] = {vl.x, vl.y, vl.z, vl.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const float d0 = v[8 * u + 2 * k], d1 = v[8 * u + 2 * k + 1];
-              const float2 fa = unpack2(wa[k], a.bf16), fb = unpack2(wb[k], a.bf16);
-              wa[k] = pack2(d0 * fa.x, d1 * fa.y, a.bf16);
-              wb[k] = pack2(d0 * fb.x, d1 * fb.y, a.bf16);
+              // upper half in bytes 2 and 3, low byte in byte 1, byte 0 cleared
+              const uint32_t lo = wl[k];
+              const float a0 = __uint_as_float(__byte_perm(wa[k], lo, 0x1040) & 0xffffff00u);
+              const float a1 = __uint_as_float(__byte_perm(wa[k], lo, 0x3260) & 0xffffff00u);
+              const float b0 = __uint_as_float(__byte_perm(wb[k], lo, 0x1050) & 0xffffff00u);
+              const float b1 = __uint_as_float(__byte_perm(wb[k], lo, 0x3270) & 0xffffff00u);
+              wa[k] = pack2(d0 * a0, d1 * a1, a.bf16);
+              wb[k] = pack2(d0 * b0, d1 * b1, a.bf16);
             }
-            *pa = *reinterpret_cast<uint4*>(wa);
-            *pb = *reinterpret_cast<uint4*>(wb);
+            *pa = make_uint4(wa[0], wa[1], wa[2], wa[3]);
+            *pb = make_uint4(wb[0], wb[1], wb[2], wb[3]);
           }
-          __syncwarp();
-          stage_to_global<64>(st0, (uint16_t*)a.du + at, a.ld_f, rows, col, pr.N, true);
-          stage_to_global<64>(st0 + 2048, (uint16_t*)a.dg + at, a.ld_f, rows, col, pr.N, true);
-          __syncwarp();
-        }
-      } else {
-        const int esz = a.out_f32 ? 4 : 2;
-        const bool vec = ((uintptr_t)pr.out & 15) == 0 && (pr.ld_out * esz) % 16 == 0;
-#pragma unroll 1
-        for (int c = half * 128; c < half * 128 + 128; c += 32) {
+          store_box(&a.mo[3], 0, col0 + c, row0);
+          store_box(&a.mo[4], 1, col0 + c, row0);
+          if (c + 128 < kCols) {
+            __syncwarp();
+            load_ab(c + 128);
+          }
+        } else {
           float v[32];
           tmem_ld32(tacc + c, v);
           tmem_wait_ld();
-          const int col = tl.nt * BN + c;
-          const int64_t at = (int64_t)row0 * pr.ld_out;
-          if (a.out_f32) {
+          if (lane == 0) bulk_wait_read<0>();
+          __syncwarp();
+          if (a.out_f32) {  // two boxes of 16 columns
 #pragma unroll
             for (int u = 0; u < 8; ++u)
-              *reinterpret_cast<float4*>(st0 + stage_off<128>(lane, u)) =
+              *reinterpret_cast<float4*>(box + (u >> 2) * kBox + box_off(lane, u & 3)) =
                   make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
-            __syncwarp();
-            stage_to_global<128>(st0, (float*)pr.out + at, pr.ld_out, rows, col, pr.N, vec);
           } else {
-            stage_row16(st0, lane, v, a.bf16);
-            __syncwarp();
-            stage_to_global<64>(st0, (uint16_t*)pr.out + at, pr.ld_out, rows, col, pr.N, vec);
+            stage_row16(box, lane, v, a.bf16);
           }
-          __syncwarp();
+          if (a.out_tma) {
+            store_box(&a.mo[tl.prob], 0, col0 + c, row0);
+            if (a.out_f32) store_box(&a.mo[tl.prob], 1, col0 + c + 16, row0);
+          } else {
+            __syncwarp();
+            const int64_t at = (int64_t)row0 * pr.ld_out;
+            if (a.out_f32) {
+              box_to_global(box, (float*)pr.out + at, pr.ld_out, rows, col0 + c, pr.N);
+              box_to_global(box + kBox, (float*)pr.out + at, pr.ld_out, rows, col0 + c + 16, pr.N);
+            } else {
+              box_to_global(box, (uint16_t*)pr.out + at, pr.ld_out, rows, col0 + c, pr.N);
+            }
+            __syncwarp();
+          }
         }
       }
+      if (lost) break;
       tc_fence_before();
-      if (lane == 0) mbar_arrive(bar[ACC_EMPTY + acc]);  // read: the MMA warp may reuse it
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_rank(bar[C::ACC_EMPTY + acc], 0));  // read: the products may reuse it
     }
+    if (lane == 0) bulk_wait_all();
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // the peer's products, copies and signals for this CTA are done
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  if (warp == 1) tmem_dealloc_pair(tmem, 2 * BN);
 }
 
 // --------------------------------------------------------------------- host
+CUtensorMapDataType map_type(int dtype) {
+  return dtype == DSALT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
 // 2-D row-major tensor [rows, cols] with row stride ld (elements), as an operand
-// whose 64 × 128 (K-major) or 64 × 64 (MN-major) boxes the kernel loads.
-bool encode(CUtensorMap* m, int dtype, const void* base, int64_t rows, int64_t cols, int64_t ld, bool mn) {
-  const CUtensorMapDataType dt = dtype == DSALT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  return encode_tensor_map_3d(m, dt, base, (uint64_t)cols, (uint64_t)rows, 1, (uint64_t)ld * 2, (uint64_t)ld * 2, 64,
-                              mn ? 64 : 128, 1) == CUDA_SUCCESS;
+// whose 64 × W (K-major) or 64 × 64 (MN-major) boxes the kernel loads.
+bool encode(CUtensorMap* m, int dtype, const void* base, int64_t rows, int64_t cols, int64_t ld, bool mn, int w) {
+  return encode_tensor_map_2d(m, map_type(dtype), base, rows, cols, (uint64_t)ld * 2, 64, mn ? 64 : w, 128) == CUDA_SUCCESS;
+}
+// the boxes that the epilogue stages: 32 rows × 64 bytes
+bool encode_box(CUtensorMap* m, int dtype, const void* base, int64_t rows, int64_t cols, int64_t ld) {
+  const bool f32 = dtype == DSALT_F32;
+  return encode_tensor_map_2d(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : map_type(dtype), base, rows, cols,
+                              (uint64_t)ld * (f32 ? 4 : 2), f32 ? 16 : 32, 32, 64) == CUDA_SUCCESS;
 }
 
 cudaError_t sm_count(int* out) {
@@ -422,15 +469,15 @@ void add_problem(Args& a, int64_t M, int64_t N, int tile_n, void* out, int64_t l
   ++a.n_prob;
 }
 
-template <bool AMN, bool BMN, int EPI>
+template <bool AMN, bool BMN, int EPI, int BN, int ACT = 0>
 cudaError_t launch(const Args& a, cudaStream_t st) {
-  auto kernel = ffn_gemm_kernel<AMN, BMN, EPI>;
-  const size_t smem = sizeof(Smem) + 1024;
+  auto kernel = ffn_gemm_kernel<AMN, BMN, EPI, BN, ACT>;
+  const size_t smem = sizeof(typename Cfg<BN, EPI>::Smem) + 1024;
   cudaError_t e = ensure_smem((const void*)kernel, smem);
   if (e != cudaSuccess) return e;
   int sms = 0;
   if ((e = sm_count(&sms)) != cudaSuccess) return e;
-  kernel<<<(unsigned)std::min(a.n_tiles, sms), kThreads, smem, st>>>(a);
+  kernel<<<(unsigned)(2 * std::min(a.n_tiles, sms / 2)), kThreads, smem, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -439,57 +486,79 @@ Args base_args(const DsaltGatedFfnParams& p) {
   memset(&a, 0, sizeof(a));
   a.bf16 = p.dtype == DSALT_BF16;
   a.n_seg = 1;
-  a.act = p.activation;
-  a.ld_f = p.ld_f;
   a.status = p.status;
   return a;
+}
+// results of the plain products: tensor maps where their rows are 16-byte aligned
+bool encode_out(Args& a, int dtype) {
+  const int es = dtype == DSALT_F32 ? 4 : 2;
+  a.out_f32 = dtype == DSALT_F32;
+  a.out_tma = true;
+  for (int i = 0; i < a.n_prob; ++i)
+    a.out_tma = a.out_tma && ((uintptr_t)a.prob[i].out & 15) == 0 && a.prob[i].ld_out * es % 16 == 0;
+  for (int i = 0; a.out_tma && i < a.n_prob; ++i)
+    if (!encode_box(&a.mo[i], dtype, a.prob[i].out, a.prob[i].M, a.prob[i].N, a.prob[i].ld_out)) return false;
+  return true;
 }
 
 }  // namespace ffn
 
 cudaError_t launch_ffn(int stage, const DsaltGatedFfnParams& p, cudaStream_t st) {
   using namespace ffn;
+  // the tensor maps need the device's context current on this thread, which a thread
+  // that has only allocated (a backward's first call) need not have: setting the device does it
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaSetDevice(dev);
+  if (e != cudaSuccess) return e;
   Args a = base_args(p);
   const int dt = p.dtype;
-  bool ok = true;
+  constexpr int BN = 256;
+  const cudaError_t bad = cudaErrorInvalidValue;
   switch (stage) {
     case FFN_HIDDEN:
-      ok = encode(&a.ma[0], dt, p.x, p.T, p.d, p.ld_x, false) && encode(&a.mb[0], dt, p.w_gate, p.F, p.d, p.ld_wg, false) &&
-           encode(&a.mb[1], dt, p.w_up, p.F, p.d, p.ld_wu, false);
-      if (!ok) return cudaErrorInvalidValue;
       a.K = p.d;
-      a.h = p.h;
-      a.a = p.a;
-      a.b = p.b;
-      add_problem(a, p.T, p.F, 128, nullptr, 0);
-      return launch<false, false, EPI_HIDDEN>(a, st);
+      a.keep = p.a != nullptr;
+      if (!encode(&a.ma[0], dt, p.x, p.T, p.d, p.ld_x, false, 128) ||
+          !encode(&a.mb[0], dt, p.w_gate, p.F, p.d, p.ld_wg, false, BN / 2) ||
+          !encode(&a.mb[1], dt, p.w_up, p.F, p.d, p.ld_wu, false, BN / 2) || !encode_box(&a.mo[0], dt, p.h, p.T, p.F, p.ld_f))
+        return bad;
+      if (a.keep && (!encode_box(&a.mo[1], dt, p.a, p.T, p.F, p.ld_f) || !encode_box(&a.mo[2], dt, p.b, p.T, p.F, p.ld_f) ||
+                     !encode_box(&a.mo[3], dt, p.ab, p.T, p.F, p.ld_f)))
+        return bad;
+      add_problem(a, p.T, p.F, BN / 2, nullptr, 0);
+      if (p.activation == DSALT_ACT_SILU) return launch<false, false, EPI_HIDDEN, BN, DSALT_ACT_SILU>(a, st);
+      if (p.activation == DSALT_ACT_GELU) return launch<false, false, EPI_HIDDEN, BN, DSALT_ACT_GELU>(a, st);
+      return launch<false, false, EPI_HIDDEN, BN, DSALT_ACT_GELU_TANH>(a, st);
     case FFN_OUT:
-      ok = encode(&a.ma[0], dt, p.h, p.T, p.F, p.ld_f, false) && encode(&a.mb[0], dt, p.w_down, p.d_out, p.F, p.ld_wd, false);
-      if (!ok) return cudaErrorInvalidValue;
       a.K = p.F;
       add_problem(a, p.T, p.d_out, BN, p.y, p.d_out);
-      return launch<false, false, EPI_STORE>(a, st);
-    case FFN_BWD_HIDDEN:
-      ok = encode(&a.ma[0], dt, p.dy, p.T, p.d_out, p.ld_dy, false) && encode(&a.mb[0], dt, p.w_down, p.d_out, p.F, p.ld_wd, true);
-      if (!ok) return cudaErrorInvalidValue;
+      if (!encode(&a.ma[0], dt, p.h, p.T, p.F, p.ld_f, false, 128) ||
+          !encode(&a.mb[0], dt, p.w_down, p.d_out, p.F, p.ld_wd, false, BN / 2) || !encode_out(a, dt))
+        return bad;
+      return launch<false, false, EPI_STORE, BN>(a, st);
+    case FFN_BWD_HIDDEN: {
       a.K = p.d_out;
-      a.a = p.a;
-      a.b = p.b;
-      a.dg = p.dg;
-      a.du = p.du;
+      if (!encode(&a.ma[0], dt, p.dy, p.T, p.d_out, p.ld_dy, false, 128) ||
+          !encode(&a.mb[0], dt, p.w_down, p.d_out, p.F, p.ld_wd, true, 0))
+        return bad;
+      const void* box[5] = {p.a, p.b, p.ab, p.du, p.dg};
+      for (int i = 0; i < 5; ++i)
+        if (!encode_box(&a.mo[i], dt, box[i], p.T, p.F, p.ld_f)) return bad;
       add_problem(a, p.T, p.F, BN, nullptr, 0);
-      return launch<false, true, EPI_DHIDDEN>(a, st);
+      return launch<false, true, EPI_DHIDDEN, BN>(a, st);
+    }
     case FFN_BWD_INPUT:
-      ok = encode(&a.ma[0], dt, p.dg, p.T, p.F, p.ld_f, false) && encode(&a.ma[1], dt, p.du, p.T, p.F, p.ld_f, false) &&
-           encode(&a.mb[0], dt, p.w_gate, p.F, p.d, p.ld_wg, true) && encode(&a.mb[1], dt, p.w_up, p.F, p.d, p.ld_wu, true);
-      if (!ok) return cudaErrorInvalidValue;
       a.K = p.F;
       a.n_seg = 2;
       add_problem(a, p.T, p.d, BN, p.dx, p.d);
-      return launch<false, true, EPI_STORE>(a, st);
+      if (!encode(&a.ma[0], dt, p.dg, p.T, p.F, p.ld_f, false, 128) || !encode(&a.ma[1], dt, p.du, p.T, p.F, p.ld_f, false, 128) ||
+          !encode(&a.mb[0], dt, p.w_gate, p.F, p.d, p.ld_wg, true, 0) || !encode(&a.mb[1], dt, p.w_up, p.F, p.d, p.ld_wu, true, 0) ||
+          !encode_out(a, dt))
+        return bad;
+      return launch<false, true, EPI_STORE, BN>(a, st);
     case FFN_BWD_WEIGHTS: {
       a.K = (int)p.T;
-      a.out_f32 = p.w_grad_f32 != 0;
       struct { const void* l; int64_t nl, ldl; const void* r; int64_t nr, ldr; void* out; } job[3] = {
           {p.dg, p.F, p.ld_f, p.x, p.d, p.ld_x, p.dw_gate},
           {p.du, p.F, p.ld_f, p.x, p.d, p.ld_x, p.dw_up},
@@ -497,15 +566,16 @@ cudaError_t launch_ffn(int stage, const DsaltGatedFfnParams& p, cudaStream_t st)
       for (const auto& j : job) {
         if (!j.out) continue;
         const int i = a.n_prob;
-        if (!encode(&a.ma[i], dt, j.l, p.T, j.nl, j.ldl, true) || !encode(&a.mb[i], dt, j.r, p.T, j.nr, j.ldr, true))
-          return cudaErrorInvalidValue;
+        if (!encode(&a.ma[i], dt, j.l, p.T, j.nl, j.ldl, true, 0) || !encode(&a.mb[i], dt, j.r, p.T, j.nr, j.ldr, true, 0))
+          return bad;
         add_problem(a, j.nl, j.nr, BN, j.out, j.nr);
       }
       if (a.n_prob == 0) return cudaSuccess;
-      return launch<true, true, EPI_STORE>(a, st);
+      if (!encode_out(a, p.w_grad_f32 ? DSALT_F32 : dt)) return bad;
+      return launch<true, true, EPI_STORE, BN>(a, st);
     }
   }
-  return cudaErrorInvalidValue;
+  return bad;
 }
 
 }  // namespace dsalt

@@ -142,8 +142,8 @@ class GqaReduceParams(ctypes.Structure):
 
 class GatedFfnParams(ctypes.Structure):
     _fields_ = [("x", _c_void_p), ("w_gate", _c_void_p), ("w_up", _c_void_p), ("w_down", _c_void_p),
-                ("h", _c_void_p), ("a", _c_void_p), ("b", _c_void_p), ("y", _c_void_p), ("dy", _c_void_p),
-                ("dg", _c_void_p), ("du", _c_void_p), ("dx", _c_void_p), ("dw_gate", _c_void_p),
+                ("h", _c_void_p), ("a", _c_void_p), ("b", _c_void_p), ("ab", _c_void_p), ("y", _c_void_p),
+                ("dy", _c_void_p), ("dg", _c_void_p), ("du", _c_void_p), ("dx", _c_void_p), ("dw_gate", _c_void_p),
                 ("dw_up", _c_void_p), ("dw_down", _c_void_p), ("status", _c_void_p), ("T", _i64),
                 ("ld_x", _i64), ("ld_wg", _i64), ("ld_wu", _i64), ("ld_wd", _i64), ("ld_f", _i64), ("ld_dy", _i64),
                 ("d", _i32), ("F", _i32), ("d_out", _i32), ("activation", _i32), ("dtype", _i32),

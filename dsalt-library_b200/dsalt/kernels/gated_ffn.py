@@ -6,9 +6,9 @@ bf16 with fp32 accumulation.  Both projections, the activation and the product a
 one kernel: neither ``gate(x)`` nor ``up(x)`` is written to memory.  A forward that
 needs gradients also keeps ``a = act(g)`` and ``b = u·act'(g)``, from which the
 backward forms ``du = dh·a`` and ``dg = dh·b`` in the epilogue of the product that
-makes ``dh``.  Results are rounded once from the fp32 sums; only ``h`` (the operand
-of the second product) and, in the backward, ``a``, ``b``, ``dg`` and ``du`` are
-rounded on the way.
+makes ``dh``.  Results are rounded once from the fp32 sums; on the way only the
+operands of a further product are rounded to 16 bits, ``h``, ``dg`` and ``du``
+(``a`` and ``b`` are kept to 24 bits).
 
 ``swiglu_ffn`` computes the same block with library GEMMs around an activation
 kernel, with torch's rounding at every step.
@@ -50,14 +50,14 @@ def _params(x2, wg, wu, wd, activation: int, dtype: torch.dtype):
 
 
 def _forward(x2, wg, wu, wd, activation: int, dtype: torch.dtype, keep: bool):
-    """``(y, h, a, b)``; ``a`` and ``b`` only with ``keep``."""
+    """``(y, h, a, b, ab)``; the last three, 16-bit words, only with ``keep``."""
     p = _params(x2, wg, wu, wd, activation, dtype)
     dev = x2[0].device
-    h, a, b = (torch.empty(p.T, p.ld_f, dtype=dtype, device=dev) if i == 0 or keep else None for i in range(3))
+    h, a, b, ab = (torch.empty(p.T, p.ld_f, dtype=dtype, device=dev) if i == 0 or keep else None for i in range(4))
     y = torch.empty(p.T, p.d_out, dtype=dtype, device=dev)
-    p.h, p.a, p.b, p.y = h.data_ptr(), _ext.ptr(a), _ext.ptr(b), y.data_ptr()
+    p.h, p.a, p.b, p.ab, p.y = h.data_ptr(), _ext.ptr(a), _ext.ptr(b), _ext.ptr(ab), y.data_ptr()
     _ext.call_on(dev, ("dsalt_gated_ffn_hidden", "dsalt_gated_ffn_out"), p)
-    return y, h, a, b
+    return y, h, a, b, ab
 
 
 class GatedFFNFunction(torch.autograd.Function):
@@ -66,8 +66,8 @@ class GatedFFNFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation: int, dtype: torch.dtype):
         ops = [_operand(t.detach(), dtype) for t in (x, w_gate, w_up, w_down)]
-        y, h, a, b = _forward(*ops, activation, dtype, True)
-        ctx.save_for_backward(*(t for t, _ in ops), h, a, b)
+        y, *kept = _forward(*ops, activation, dtype, True)
+        ctx.save_for_backward(*(t for t, _ in ops), *kept)
         ctx.strides = [ld for _, ld in ops]
         ctx.activation, ctx.dtype = activation, dtype
         ctx.dtypes = [t.dtype for t in (x, w_gate, w_up, w_down)]
@@ -76,12 +76,12 @@ class GatedFFNFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        *ops, h, a, b = ctx.saved_tensors
+        *ops, h, a, b, ab = ctx.saved_tensors
         dtype, dev = ctx.dtype, h.device
         p = _params(*zip(ops, ctx.strides), ctx.activation, dtype)
         dy_, p.ld_dy = _operand(dy, dtype)
         need_x, *need_w = ctx.needs_input_grad[:4]
-        p.h, p.a, p.b, p.dy = h.data_ptr(), a.data_ptr(), b.data_ptr(), dy_.data_ptr()
+        p.h, p.a, p.b, p.ab, p.dy = h.data_ptr(), a.data_ptr(), b.data_ptr(), ab.data_ptr(), dy_.data_ptr()
         stages = []
         if need_x or need_w[0] or need_w[1]:
             dg, du = torch.empty_like(a), torch.empty_like(a)

@@ -495,8 +495,10 @@ DSALT_API int dsalt_swiglu_bwd(const DsaltSwigluParams* p, void* stream);
  *   g = x·Wgᵀ, u = x·Wuᵀ, h = act(g)⊙u, y = h·Wdᵀ
  * (dsalt/modules/dsalt_transformer.py:10-21 with act = silu), as five stages that
  * read their operands in place (row-major, row strides ld_*):
- *   hidden       h, and for a later backward a = act(g), b = u⊙act'(g) (both or
- *                neither), each rounded once from fp32; g and u are not stored
+ *   hidden       h, rounded once from fp32, and for a later backward a = act(g) and
+ *                b = u⊙act'(g) as the upper 24 bits of their fp32 values: the upper 16
+ *                in a and b, the next 8 of each in the low and high byte of ab (all
+ *                three or none); g and u are not stored
  *   out          y
  *   bwd_hidden   dh = dy·Wd (kept in fp32), du = R(dh⊙a), dg = R(dh⊙b)
  *   bwd_input    dx = R(dg·Wg + du·Wu), one accumulation
@@ -511,8 +513,9 @@ typedef struct DsaltGatedFfnParams {
   const void* w_up;           /* [F, d] stride ld_wu */
   const void* w_down;         /* [d_out, F] stride ld_wd */
   void* h;                    /* [T, F] stride ld_f */
-  void* a;                    /* [T, F] stride ld_f, or NULL (inference) */
-  void* b;                    /* [T, F] stride ld_f, or NULL */
+  void* a;                    /* [T, F] 16-bit words, stride ld_f, or NULL (inference) */
+  void* b;                    /* likewise */
+  void* ab;                   /* likewise */
   void* y;                    /* [T, d_out] */
   const void* dy;             /* [T, d_out] stride ld_dy        (backward) */
   void* dg;                   /* [T, F] stride ld_f */

@@ -253,12 +253,12 @@ def test_results_end_where_the_tensors_end():
     T, d, F = 130, 40, 72
     x, wg, wu, wd, dy = inputs(T, d, F, d, torch.bfloat16, grad=False)
     mark = 7.0
-    f = [torch.full((T + 4, 80), mark, device="cuda", dtype=torch.bfloat16) for _ in range(5)]
+    f = [torch.full((T + 4, 80), mark, device="cuda", dtype=torch.bfloat16) for _ in range(6)]
     y, dx = (torch.full((T + 4, d), mark, device="cuda", dtype=torch.bfloat16) for _ in range(2))
     dws = [torch.full((n + 2, m), mark, device="cuda") for n, m in ((F, d), (F, d), (d, F))]
     P = _ext.ptr
-    p = _ext.GatedFfnParams(x=P(x), w_gate=P(wg), w_up=P(wu), w_down=P(wd), h=P(f[0]), a=P(f[1]), b=P(f[2]), y=P(y),
-                            dy=P(dy), dg=P(f[3]), du=P(f[4]), dx=P(dx), dw_gate=P(dws[0]), dw_up=P(dws[1]),
+    p = _ext.GatedFfnParams(x=P(x), w_gate=P(wg), w_up=P(wu), w_down=P(wd), h=P(f[0]), a=P(f[1]), b=P(f[2]), ab=P(f[5]),
+                            y=P(y), dy=P(dy), dg=P(f[3]), du=P(f[4]), dx=P(dx), dw_gate=P(dws[0]), dw_up=P(dws[1]),
                             dw_down=P(dws[2]), T=T, ld_x=d, ld_wg=d, ld_wu=d, ld_wd=F, ld_f=80, ld_dy=d, d=d, F=F,
                             d_out=d, dtype=_ext.BF16, w_grad_f32=1)
     for name in ("hidden", "out", "bwd_hidden", "bwd_input", "bwd_weights"):
