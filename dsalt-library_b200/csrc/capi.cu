@@ -7,7 +7,9 @@
 #include "tc_pair.cuh"
 
 namespace dsalt {
-static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+CUresult encode_tensor_map_3d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t d0, uint64_t d1,
+                              uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0,
+                              uint32_t box1, uint32_t box2) {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -17,13 +19,6 @@ static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
         q == cudaDriverEntryPointSuccess)
       fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
   });
-  return fn;
-}
-
-CUresult encode_tensor_map_3d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t d0, uint64_t d1,
-                              uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0,
-                              uint32_t box1, uint32_t box2) {
-  const PFN_cuTensorMapEncodeTiled_v12000 fn = tensor_map_encoder();
   if (!fn) return CUDA_ERROR_NOT_FOUND;
   cuuint64_t dims[3] = {d0, d1, d2};
   cuuint64_t strides[2] = {stride1_bytes, stride2_bytes};
@@ -31,20 +26,6 @@ CUresult encode_tensor_map_3d(CUtensorMap* m, CUtensorMapDataType dt, const void
   cuuint32_t es[3] = {1, 1, 1};
   return fn(m, dt, 3, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-}
-
-// As a 3-D map with one plane, so that the 3-D loads and stores serve it.
-CUresult encode_tensor_map_2d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t rows, uint64_t cols,
-                              uint64_t stride_bytes, uint32_t box_cols, uint32_t box_rows, int swizzle_bytes) {
-  const PFN_cuTensorMapEncodeTiled_v12000 fn = tensor_map_encoder();
-  if (!fn) return CUDA_ERROR_NOT_FOUND;
-  cuuint64_t dims[3] = {cols, rows, 1};
-  cuuint64_t strides[2] = {stride_bytes, stride_bytes};
-  cuuint32_t box[3] = {box_cols, box_rows, 1};
-  cuuint32_t es[3] = {1, 1, 1};
-  return fn(m, dt, 3, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 }  // namespace dsalt
 

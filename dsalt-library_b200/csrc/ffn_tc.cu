@@ -26,10 +26,14 @@
 //               barrier counts both CTAs' bytes
 //   warp 1      TMEM owner; in the leader the single-thread MMA issuer
 //   warps 2-17  epilogue: TMEM lane quadrant warp % 4, every fourth 32-column chunk;
-//               results go through 64-byte-swizzled staging and TMA stores
+//               a lane owns a row, so results are staged in shared memory and copied
+//               with row-contiguous 16-byte accesses (TMA stores of the same 64-byte
+//               rows shared the TMA unit with the operands' loads: hidden 175 us
+//               instead of HIDDEN_US at T = 16384, d = 1024, F = 2816)
 // Every wait is bounded (sm100::mbar_wait).
 #include <algorithm>
 #include <cstring>
+#include <initializer_list>
 
 #include "ffn.cuh"
 #include "tc_pair.cuh"
@@ -51,7 +55,7 @@ struct Cfg {
   static constexpr int kBoxes = EPI == EPI_DHIDDEN ? 3 : 2;     // staged boxes of a warp
   static constexpr int kStages = BN == 256 ? (EPI == EPI_DHIDDEN ? 4 : 5) : 6;
   static constexpr int FULL = 0, EMPTY = kStages, ACC_FULL = 2 * kStages, ACC_EMPTY = ACC_FULL + 2,
-                       FINAL = ACC_EMPTY + 2, LOADED = FINAL + 1, NB = LOADED + kEpiWarps;
+                       FINAL = ACC_EMPTY + 2, NB = FINAL + 1;
   struct alignas(1024) Smem {
     uint8_t ring[kStages][kStageBytes];
     uint8_t stage[kEpiWarps][kBoxes * kBox];
@@ -70,10 +74,11 @@ struct Problem {
 
 struct alignas(64) Args {
   CUtensorMap ma[kMaxProb], mb[kMaxProb];  // per problem, or per K segment of the only problem
-  CUtensorMap mo[5];                       // store: out of each problem; hidden: h, a, b, ab; dhidden: a, b, ab, du, dg
   Problem prob[kMaxProb];
   int n_prob, n_seg, K, n_tiles;
-  bool bf16, out_f32, out_tma, keep;
+  bool bf16, out_f32, out_vec, keep;
+  uint16_t* f[5];  // [T, F] stride ld_f: hidden writes h, a, b, ab; dhidden reads a, b, ab, writes du, dg
+  int64_t ld_f;
   int32_t* status;
 };
 
@@ -116,35 +121,50 @@ __device__ __forceinline__ void act_pair(float g, float& a, float& da) {
 }
 
 // ------------------------------------------------------------------- staging
-// A box of 32 rows × 64 bytes in TMA's 64-byte swizzle (16-byte units XORed with
-// row / 2 % 4): a row's owner writes its four units without bank conflicts.
+// A box of 32 rows × 64 bytes, its 16-byte units XORed with row / 2 % 4: a row's owner
+// writes or reads its four units, and four lanes copy a row, without bank conflicts.
 __device__ __forceinline__ uint32_t box_off(int row, int u) { return row * 64 + ((u ^ ((row >> 1) & 3)) << 4); }
 
-// this lane's row of 32 values, rounded to 16 bits
-__device__ __forceinline__ void stage_row16(uint8_t* box, int lane, const float* v, bool bf16) {
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    *reinterpret_cast<uint4*>(box + box_off(lane, u)) =
-        make_uint4(sm100::pack2(v[8 * u + 0], v[8 * u + 1], bf16), sm100::pack2(v[8 * u + 2], v[8 * u + 3], bf16),
-                   sm100::pack2(v[8 * u + 4], v[8 * u + 5], bf16), sm100::pack2(v[8 * u + 6], v[8 * u + 7], bf16));
-}
 __device__ __forceinline__ void stage_words(uint8_t* box, int lane, const uint32_t* w) {
 #pragma unroll
   for (int u = 0; u < 4; ++u)
     *reinterpret_cast<uint4*>(box + box_off(lane, u)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
 }
-// a staged box → global rows and columns inside [rows, N), element by element: results
-// whose rows are not 16-byte aligned (no tensor map describes them)
+// A staged box → global rows [0, rows) at `out`, `cols` columns: 16-byte accesses, of
+// which the last may reach past `cols` (the rows' padding to 8 elements).
 template <typename E>
-__device__ __forceinline__ void box_to_global(const uint8_t* box, E* out, int64_t ld, int rows, int c0, int N) {
+__device__ __forceinline__ void box_to_rows(const uint8_t* box, E* out, int64_t ld, int rows, int cols) {
+  constexpr int kE = 16 / sizeof(E);
+  const int lane = threadIdx.x & 31, r = lane >> 2, u = lane & 3;
+  if (u * kE >= cols) return;
+  out += r * ld + u * kE;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    if (r + i < rows) *reinterpret_cast<uint4*>(out + i * ld) = *reinterpret_cast<const uint4*>(box + box_off(r + i, u));
+}
+// the same element by element, for results whose rows are not 16-byte aligned
+template <typename E>
+__device__ __forceinline__ void box_to_elements(const uint8_t* box, E* out, int64_t ld, int rows, int cols) {
   constexpr int kCols = 64 / sizeof(E);
-  const int lane = threadIdx.x & 31;
-  for (int i = lane; i < 32 * kCols; i += 32) {
+  for (int i = threadIdx.x & 31; i < 32 * kCols; i += 32) {
     const int row = i / kCols, c = i % kCols;
-    if (row < rows && c0 + c < N)
-      out[row * ld + c0 + c] = *reinterpret_cast<const E*>(box + box_off(row, c * (int)sizeof(E) / 16) + c * sizeof(E) % 16);
+    if (row < rows && c < cols)
+      out[row * ld + c] = *reinterpret_cast<const E*>(box + box_off(row, c * (int)sizeof(E) / 16) + c * sizeof(E) % 16);
   }
 }
+// global rows → a box, asynchronously (zeros outside); cp_async_wait before reading it
+__device__ __forceinline__ void rows_to_box(uint32_t box, const uint16_t* in, int64_t ld, int rows, int cols) {
+  const int lane = threadIdx.x & 31, r = lane >> 2, u = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    const bool on = r + i < rows && u * 8 < cols;
+    const uint16_t* src = on ? in + (r + i) * ld + u * 8 : in;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(box + box_off(r + i, u)), "l"(src), "r"(on ? 16 : 0)
+                 : "memory");
+  }
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 // bytes 2 and 3 of two words: the upper 16 bits of fp32 x (low half) and y
 __device__ __forceinline__ uint32_t upper16(float x, float y) {
   return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
@@ -189,7 +209,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) ffn_gem
       mbar_init(bar[C::ACC_EMPTY + b], 2 * kEpiWarps);
     }
     mbar_init(bar[C::FINAL], 1);
-    for (int w = 0; w < kEpiWarps; ++w) mbar_init(bar[C::LOADED + w], 1);
     fence_mbar_init();
     sm.abort_flag = 0;
   }
@@ -266,44 +285,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) ffn_gem
     const uint32_t lane_addr = (uint32_t)(32 * q4) << 16;
     uint8_t* box = sm.stage[warp - 2];
     const uint32_t box_u32 = smem_u32(box);
-    int li = 0, loads = 0;
-    // a box that this warp staged → its place in global memory
-    auto store_box = [&](const CUtensorMap* map, int i, int col, int row) {
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        tma_store_3d(map, box_u32 + i * kBox, col, row, 0);
-        bulk_commit();
-      }
-    };
+    constexpr int kCols = EPI == EPI_HIDDEN ? BN / 2 : BN;  // result columns of a tile
+    int li = 0;
     for (int t = t0; t < a.n_tiles; t += t_step, ++li) {
       const Tile tl = decode(a, t);
       const Problem& pr = a.prob[tl.prob];
       const int acc = li & 1;
       const int row0 = tl.m0 + 128 * (int)rank + 32 * q4, rows = pr.M - row0;  // rows of this warp (may be <= 0)
-      constexpr int kCols = EPI == EPI_HIDDEN ? BN / 2 : BN;                   // result columns of a tile
-      const int col0 = tl.nt * kCols;
+      const int col0 = tl.nt * kCols, cols = pr.N - col0;
+      const int64_t at = EPI == EPI_STORE ? row0 * pr.ld_out + col0 : row0 * a.ld_f + col0;
       auto load_ab = [&](int c) {  // the a, b and ab boxes of columns c (dhidden)
-        if (lane == 0) {
-          bulk_wait_read<0>();  // the boxes' last results are out
-          mbar_expect_tx(bar[C::LOADED + warp - 2], 3 * kBox);
 #pragma unroll
-          for (int i = 0; i < 3; ++i)
-            tma_load_3d(box_u32 + i * kBox, &a.mo[i], bar[C::LOADED + warp - 2], col0 + c, row0, 0);
-        }
+        for (int i = 0; i < 3; ++i) rows_to_box(box_u32 + i * kBox, rows > 0 ? a.f[i] + at + c : a.f[i], a.ld_f, rows, cols - c);
+        cp_async_commit();
       };
-      if constexpr (EPI == EPI_DHIDDEN)
+      if constexpr (EPI == EPI_DHIDDEN)  // on the way while the products finish
         if (cg * 32 < kCols) load_ab(cg * 32);
-      const bool full = mbar_wait(bar[C::ACC_FULL + acc], (li >> 1) & 1, abort_flag, a.status);
-      if (!__all_sync(0xffffffffu, full)) {
-        if (EPI == EPI_DHIDDEN && cg * 32 < kCols && lane == 0) mbar_drain(bar[C::LOADED + warp - 2], loads & 1);
-        break;
-      }
+      if (!__all_sync(0xffffffffu, mbar_wait(bar[C::ACC_FULL + acc], (li >> 1) & 1, abort_flag, a.status))) break;
       tc_fence_after();
       const uint32_t tacc = tmem + acc * BN + lane_addr;
-      bool lost = false;
+      auto release = [&]() {  // this warp has read its part: the products may reuse the accumulator
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_rank(bar[C::ACC_EMPTY + acc], 0));
+      };
 #pragma unroll 1
       for (int c = cg * 32; c < kCols; c += 128) {
+        const bool last = c + 128 >= kCols;
         if constexpr (EPI == EPI_HIDDEN) {
           uint32_t wh[16], wa[16], wb[16], wl[16];
 #pragma unroll
@@ -312,6 +320,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) ffn_gem
             tmem_ld16(tacc + c + c2, g);
             tmem_ld16(tacc + BN / 2 + c + c2, u);
             tmem_wait_ld();
+            if (last && c2 == 16) release();
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
               float a0, a1, d0, d1;
@@ -328,31 +337,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) ffn_gem
                                   __byte_perm(__float_as_uint(a1), __float_as_uint(d1), 0x0051), 0x5410);
             }
           }
-          if (lane == 0) bulk_wait_read<0>();
-          __syncwarp();
           stage_words(box, lane, wh);
-          store_box(&a.mo[0], 0, col0 + c, row0);
+          stage_words(box + kBox, lane, wa);
+          __syncwarp();
+          box_to_rows(box, a.f[0] + at + c, a.ld_f, rows, cols - c);
           if (a.keep) {
-            stage_words(box + kBox, lane, wa);
-            store_box(&a.mo[1], 1, col0 + c, row0);
-            if (lane == 0) bulk_wait_read<1>();
+            box_to_rows(box + kBox, a.f[1] + at + c, a.ld_f, rows, cols - c);
             __syncwarp();
             stage_words(box, lane, wb);
-            store_box(&a.mo[2], 0, col0 + c, row0);
-            if (lane == 0) bulk_wait_read<1>();
-            __syncwarp();
             stage_words(box + kBox, lane, wl);
-            store_box(&a.mo[3], 1, col0 + c, row0);
+            __syncwarp();
+            box_to_rows(box, a.f[2] + at + c, a.ld_f, rows, cols - c);
+            box_to_rows(box + kBox, a.f[3] + at + c, a.ld_f, rows, cols - c);
           }
+          __syncwarp();
         } else if constexpr (EPI == EPI_DHIDDEN) {
           float v[32];
           tmem_ld32(tacc + c, v);
+          cp_async_wait();
           tmem_wait_ld();
-          if (!__all_sync(0xffffffffu, mbar_wait(bar[C::LOADED + warp - 2], loads & 1, abort_flag, a.status))) {
-            lost = true;
-            break;
-          }
-          ++loads;
+          if (last) release();
+          __syncwarp();
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             uint4* pa = reinterpret_cast<uint4*>(box + box_off(lane, u));
@@ -375,48 +380,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) ffn_gem
             *pa = make_uint4(wa[0], wa[1], wa[2], wa[3]);
             *pb = make_uint4(wb[0], wb[1], wb[2], wb[3]);
           }
-          store_box(&a.mo[3], 0, col0 + c, row0);
-          store_box(&a.mo[4], 1, col0 + c, row0);
-          if (c + 128 < kCols) {
-            __syncwarp();
-            load_ab(c + 128);
-          }
+          __syncwarp();
+          box_to_rows(box, a.f[3] + at + c, a.ld_f, rows, cols - c);
+          box_to_rows(box + kBox, a.f[4] + at + c, a.ld_f, rows, cols - c);
+          __syncwarp();
+          if (c + 128 < kCols) load_ab(c + 128);
         } else {
           float v[32];
           tmem_ld32(tacc + c, v);
           tmem_wait_ld();
-          if (lane == 0) bulk_wait_read<0>();
-          __syncwarp();
+          if (last) release();
           if (a.out_f32) {  // two boxes of 16 columns
 #pragma unroll
             for (int u = 0; u < 8; ++u)
               *reinterpret_cast<float4*>(box + (u >> 2) * kBox + box_off(lane, u & 3)) =
                   make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
-          } else {
-            stage_row16(box, lane, v, a.bf16);
-          }
-          if (a.out_tma) {
-            store_box(&a.mo[tl.prob], 0, col0 + c, row0);
-            if (a.out_f32) store_box(&a.mo[tl.prob], 1, col0 + c + 16, row0);
-          } else {
             __syncwarp();
-            const int64_t at = (int64_t)row0 * pr.ld_out;
-            if (a.out_f32) {
-              box_to_global(box, (float*)pr.out + at, pr.ld_out, rows, col0 + c, pr.N);
-              box_to_global(box + kBox, (float*)pr.out + at, pr.ld_out, rows, col0 + c + 16, pr.N);
+            float* out = (float*)pr.out + at + c;
+            if (a.out_vec) {
+              box_to_rows(box, out, pr.ld_out, rows, cols - c);
+              box_to_rows(box + kBox, out + 16, pr.ld_out, rows, cols - c - 16);
             } else {
-              box_to_global(box, (uint16_t*)pr.out + at, pr.ld_out, rows, col0 + c, pr.N);
+              box_to_elements(box, out, pr.ld_out, rows, cols - c);
+              box_to_elements(box + kBox, out + 16, pr.ld_out, rows, cols - c - 16);
             }
+          } else {
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], a.bf16);
+            stage_words(box, lane, w);
             __syncwarp();
+            uint16_t* out = (uint16_t*)pr.out + at + c;
+            if (a.out_vec) box_to_rows(box, out, pr.ld_out, rows, cols - c);
+            else box_to_elements(box, out, pr.ld_out, rows, cols - c);
           }
+          __syncwarp();
         }
       }
-      if (lost) break;
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_rank(bar[C::ACC_EMPTY + acc], 0));  // read: the products may reuse it
+      if (cg * 32 >= kCols) release();
     }
-    if (lane == 0) bulk_wait_all();
+    cp_async_wait();
   }
   __syncwarp();
   tc_fence_before();
@@ -433,15 +436,9 @@ CUtensorMapDataType map_type(int dtype) {
 // 2-D row-major tensor [rows, cols] with row stride ld (elements), as an operand
 // whose 64 × W (K-major) or 64 × 64 (MN-major) boxes the kernel loads.
 bool encode(CUtensorMap* m, int dtype, const void* base, int64_t rows, int64_t cols, int64_t ld, bool mn, int w) {
-  return encode_tensor_map_2d(m, map_type(dtype), base, rows, cols, (uint64_t)ld * 2, 64, mn ? 64 : w, 128) == CUDA_SUCCESS;
+  return encode_tensor_map_3d(m, map_type(dtype), base, (uint64_t)cols, (uint64_t)rows, 1, (uint64_t)ld * 2, (uint64_t)ld * 2,
+                              64, mn ? 64 : w, 1) == CUDA_SUCCESS;
 }
-// the boxes that the epilogue stages: 32 rows × 64 bytes
-bool encode_box(CUtensorMap* m, int dtype, const void* base, int64_t rows, int64_t cols, int64_t ld) {
-  const bool f32 = dtype == DSALT_F32;
-  return encode_tensor_map_2d(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : map_type(dtype), base, rows, cols,
-                              (uint64_t)ld * (f32 ? 4 : 2), f32 ? 16 : 32, 32, 64) == CUDA_SUCCESS;
-}
-
 cudaError_t sm_count(int* out) {
   static int counts[64] = {};
   int dev = 0;
@@ -486,19 +483,20 @@ Args base_args(const DsaltGatedFfnParams& p) {
   memset(&a, 0, sizeof(a));
   a.bf16 = p.dtype == DSALT_BF16;
   a.n_seg = 1;
+  a.ld_f = p.ld_f;
   a.status = p.status;
   return a;
 }
-// results of the plain products: tensor maps where their rows are 16-byte aligned
-bool encode_out(Args& a, int dtype) {
-  const int es = dtype == DSALT_F32 ? 4 : 2;
-  a.out_f32 = dtype == DSALT_F32;
-  a.out_tma = true;
+void set_f(Args& a, std::initializer_list<void*> f) {
+  int i = 0;
+  for (void* q : f) a.f[i++] = reinterpret_cast<uint16_t*>(q);
+}
+// the type of the plain products' results, and whether their rows take 16-byte stores
+void set_out(Args& a, bool f32) {
+  a.out_f32 = f32;
+  a.out_vec = true;
   for (int i = 0; i < a.n_prob; ++i)
-    a.out_tma = a.out_tma && ((uintptr_t)a.prob[i].out & 15) == 0 && a.prob[i].ld_out * es % 16 == 0;
-  for (int i = 0; a.out_tma && i < a.n_prob; ++i)
-    if (!encode_box(&a.mo[i], dtype, a.prob[i].out, a.prob[i].M, a.prob[i].N, a.prob[i].ld_out)) return false;
-  return true;
+    a.out_vec = a.out_vec && ((uintptr_t)a.prob[i].out & 15) == 0 && a.prob[i].ld_out * (f32 ? 4 : 2) % 16 == 0;
 }
 
 }  // namespace ffn
@@ -521,11 +519,9 @@ cudaError_t launch_ffn(int stage, const DsaltGatedFfnParams& p, cudaStream_t st)
       a.keep = p.a != nullptr;
       if (!encode(&a.ma[0], dt, p.x, p.T, p.d, p.ld_x, false, 128) ||
           !encode(&a.mb[0], dt, p.w_gate, p.F, p.d, p.ld_wg, false, BN / 2) ||
-          !encode(&a.mb[1], dt, p.w_up, p.F, p.d, p.ld_wu, false, BN / 2) || !encode_box(&a.mo[0], dt, p.h, p.T, p.F, p.ld_f))
+          !encode(&a.mb[1], dt, p.w_up, p.F, p.d, p.ld_wu, false, BN / 2))
         return bad;
-      if (a.keep && (!encode_box(&a.mo[1], dt, p.a, p.T, p.F, p.ld_f) || !encode_box(&a.mo[2], dt, p.b, p.T, p.F, p.ld_f) ||
-                     !encode_box(&a.mo[3], dt, p.ab, p.T, p.F, p.ld_f)))
-        return bad;
+      set_f(a, {p.h, p.a, p.b, p.ab});
       add_problem(a, p.T, p.F, BN / 2, nullptr, 0);
       if (p.activation == DSALT_ACT_SILU) return launch<false, false, EPI_HIDDEN, BN, DSALT_ACT_SILU>(a, st);
       if (p.activation == DSALT_ACT_GELU) return launch<false, false, EPI_HIDDEN, BN, DSALT_ACT_GELU>(a, st);
@@ -534,28 +530,26 @@ cudaError_t launch_ffn(int stage, const DsaltGatedFfnParams& p, cudaStream_t st)
       a.K = p.F;
       add_problem(a, p.T, p.d_out, BN, p.y, p.d_out);
       if (!encode(&a.ma[0], dt, p.h, p.T, p.F, p.ld_f, false, 128) ||
-          !encode(&a.mb[0], dt, p.w_down, p.d_out, p.F, p.ld_wd, false, BN / 2) || !encode_out(a, dt))
+          !encode(&a.mb[0], dt, p.w_down, p.d_out, p.F, p.ld_wd, false, BN / 2))
         return bad;
+      set_out(a, false);
       return launch<false, false, EPI_STORE, BN>(a, st);
-    case FFN_BWD_HIDDEN: {
+    case FFN_BWD_HIDDEN:
       a.K = p.d_out;
       if (!encode(&a.ma[0], dt, p.dy, p.T, p.d_out, p.ld_dy, false, 128) ||
           !encode(&a.mb[0], dt, p.w_down, p.d_out, p.F, p.ld_wd, true, 0))
         return bad;
-      const void* box[5] = {p.a, p.b, p.ab, p.du, p.dg};
-      for (int i = 0; i < 5; ++i)
-        if (!encode_box(&a.mo[i], dt, box[i], p.T, p.F, p.ld_f)) return bad;
+      set_f(a, {p.a, p.b, p.ab, p.du, p.dg});
       add_problem(a, p.T, p.F, BN, nullptr, 0);
       return launch<false, true, EPI_DHIDDEN, BN>(a, st);
-    }
     case FFN_BWD_INPUT:
       a.K = p.F;
       a.n_seg = 2;
       add_problem(a, p.T, p.d, BN, p.dx, p.d);
       if (!encode(&a.ma[0], dt, p.dg, p.T, p.F, p.ld_f, false, 128) || !encode(&a.ma[1], dt, p.du, p.T, p.F, p.ld_f, false, 128) ||
-          !encode(&a.mb[0], dt, p.w_gate, p.F, p.d, p.ld_wg, true, 0) || !encode(&a.mb[1], dt, p.w_up, p.F, p.d, p.ld_wu, true, 0) ||
-          !encode_out(a, dt))
+          !encode(&a.mb[0], dt, p.w_gate, p.F, p.d, p.ld_wg, true, 0) || !encode(&a.mb[1], dt, p.w_up, p.F, p.d, p.ld_wu, true, 0))
         return bad;
+      set_out(a, false);
       return launch<false, true, EPI_STORE, BN>(a, st);
     case FFN_BWD_WEIGHTS: {
       a.K = (int)p.T;
@@ -571,7 +565,7 @@ cudaError_t launch_ffn(int stage, const DsaltGatedFfnParams& p, cudaStream_t st)
         add_problem(a, j.nl, j.nr, BN, j.out, j.nr);
       }
       if (a.n_prob == 0) return cudaSuccess;
-      if (!encode_out(a, p.w_grad_f32 ? DSALT_F32 : dt)) return bad;
+      set_out(a, p.w_grad_f32 != 0);
       return launch<true, true, EPI_STORE, BN>(a, st);
     }
   }

@@ -21,9 +21,11 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// arrive on a barrier of any CTA of the cluster (address from map_rank)
+// Arrive on a barrier of any CTA of the cluster (address from map_rank).  For TMEM
+// reads, which the tcgen05 fences order: no cluster-scope release, which would wait for
+// every global store of the warp.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // TMA load into this CTA's shared memory whose bytes are counted by `bar`, a barrier
 // of either CTA of the pair (address from map_rank)
@@ -56,11 +58,6 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
       ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
-// until at most N of this thread's committed bulk stores still read shared memory
-template <int N>
-__device__ __forceinline__ void bulk_wait_read() {
-  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ float fast_rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -69,8 +66,4 @@ __device__ __forceinline__ float fast_rcp(float x) {
 
 }  // namespace sm100
 
-// cuTensorMapEncodeTiled of a row-major [rows, cols] tensor (row stride in bytes) with
-// boxes of box_cols × box_rows; swizzle_bytes 64 or 128 = the box's row bytes.
-CUresult encode_tensor_map_2d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t rows, uint64_t cols,
-                              uint64_t stride_bytes, uint32_t box_cols, uint32_t box_rows, int swizzle_bytes);
 }  // namespace dsalt
