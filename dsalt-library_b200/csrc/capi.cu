@@ -4,7 +4,7 @@
 #include <mutex>
 
 #include "ffn.cuh"
-#include "tc_pair.cuh"
+#include "sm100.cuh"
 
 namespace dsalt {
 CUresult encode_tensor_map_3d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t d0, uint64_t d1,
@@ -396,8 +396,8 @@ int dsalt_gqa_reduce(const DsaltGqaReduceParams* p, void* stream) {
   return status_of(launch_gqa_reduce(*p, (cudaStream_t)stream));
 }
 
-// Sizes and the operands that a stage reads and writes; every stride covers its row.
-static int check_ffn(const DsaltGatedFfnParams* p, int stage) {
+// Sizes, strides and the operands that a direction reads and writes.
+static int check_ffn(const DsaltGatedFfnParams* p, bool bwd) {
   if (!p || p->T < 0 || p->d <= 0 || p->F <= 0 || p->d_out <= 0) return DSALT_ERR_ARG;
   if (p->dtype != DSALT_F16 && p->dtype != DSALT_BF16) return DSALT_ERR_DTYPE;
   if (p->activation < DSALT_ACT_SILU || p->activation > DSALT_ACT_GELU_TANH) return DSALT_ERR_ARG;
@@ -407,58 +407,60 @@ static int check_ffn(const DsaltGatedFfnParams* p, int stage) {
   const int64_t tall = p->T > p->F ? p->T : p->F, wide = p->d > p->d_out ? p->d : p->d_out;
   const int64_t cols = p->F > wide ? p->F : wide, rows = tall > wide ? tall : wide;
   if (((rows + 127) / 128) * ((cols + 127) / 128) > INT32_MAX / 4) return DSALT_ERR_TOO_LARGE;
-  struct In { const void* ptr; int64_t ld, width; };
-  const In x = {p->x, p->ld_x, p->d}, wg = {p->w_gate, p->ld_wg, p->d}, wu = {p->w_up, p->ld_wu, p->d},
-           wd = {p->w_down, p->ld_wd, p->F}, dy = {p->dy, p->ld_dy, p->d_out}, h = {p->h, p->ld_f, p->F},
-           a = {p->a, p->ld_f, p->F}, b = {p->b, p->ld_f, p->F}, ab = {p->ab, p->ld_f, p->F}, dg = {p->dg, p->ld_f, p->F}, du = {p->du, p->ld_f, p->F};
-  In need[8];
-  int n = 0;
-  switch (stage) {
-    case FFN_HIDDEN:
-      if ((p->a == nullptr) != (p->b == nullptr) || (p->a == nullptr) != (p->ab == nullptr)) return DSALT_ERR_ARG;
-      need[n++] = x; need[n++] = wg; need[n++] = wu; need[n++] = h;
-      if (p->a) { need[n++] = a; need[n++] = b; need[n++] = ab; }
-      break;
-    case FFN_OUT: need[n++] = h; need[n++] = wd; break;
-    case FFN_BWD_HIDDEN: need[n++] = dy; need[n++] = wd; need[n++] = a; need[n++] = b; need[n++] = ab; need[n++] = dg; need[n++] = du; break;
-    case FFN_BWD_INPUT: need[n++] = dg; need[n++] = du; need[n++] = wg; need[n++] = wu; break;
-    default:
-      if (p->dw_gate) need[n++] = dg;
-      if (p->dw_up) need[n++] = du;
-      if (p->dw_gate || p->dw_up) need[n++] = x;
-      if (p->dw_down) { need[n++] = dy; need[n++] = h; }
-  }
-  for (int i = 0; i < n; ++i)
-    if (need[i].ld < need[i].width || need[i].ld % 8 != 0 || need[i].ld > ((int64_t)1 << 38)) return DSALT_ERR_ARG;
+  struct Operand { const void* ptr; int64_t ld, width; bool used; };
+  const bool hidden = p->dx || p->dw_gate || p->dw_up;  // the backward forms dg and du
+  const bool kept = bwd ? hidden : p->a || p->b || p->ab;
+  const Operand all[] = {
+      {p->x, p->ld_x, p->d, !bwd || p->dw_gate || p->dw_up},
+      {p->w_gate, p->ld_wg, p->d, !bwd || p->dx},
+      {p->w_up, p->ld_wu, p->d, !bwd || p->dx},
+      {p->w_down, p->ld_wd, p->F, !bwd || hidden},
+      {p->dy, p->ld_dy, p->d_out, bwd},
+      {p->h, p->ld_f, p->F, !bwd || p->dw_down},
+      {p->a, p->ld_f, p->F, kept},
+      {p->b, p->ld_f, p->F, kept},
+      {p->ab, p->ld_f, p->F, kept},
+      {p->dg, p->ld_f, p->F, bwd && hidden},
+      {p->du, p->ld_f, p->F, bwd && hidden},
+  };
+  for (const Operand& o : all)
+    if (o.used && (o.ld < o.width || o.ld % 8 != 0 || o.ld > ((int64_t)1 << 38))) return DSALT_ERR_ARG;
   if (p->T == 0) return DSALT_OK;
-  for (int i = 0; i < n; ++i) {
-    if (!need[i].ptr) return DSALT_ERR_ARG;
-    if (!aligned16(need[i].ptr)) return DSALT_ERR_ALIGN;
+  for (const Operand& o : all) {
+    if (!o.used) continue;
+    if (!o.ptr) return DSALT_ERR_ARG;
+    if (!aligned16(o.ptr)) return DSALT_ERR_ALIGN;
   }
-  if ((stage == FFN_OUT && !p->y) || (stage == FFN_BWD_INPUT && !p->dx)) return DSALT_ERR_ARG;
-  return DSALT_OK;
+  return bwd || p->y ? DSALT_OK : DSALT_ERR_ARG;
 }
 
-static int run_ffn(const DsaltGatedFfnParams* p, int stage, void* stream) {
-  const int rc = check_ffn(p, stage);
-  if (rc != DSALT_OK) return rc;
+int dsalt_gated_ffn_fwd(const DsaltGatedFfnParams* p, void* stream) {
+  const int rc = check_ffn(p, false);
+  if (rc != DSALT_OK || p->T == 0) return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  if (p->T > 0) return status_of(launch_ffn(stage, *p, st));
-  if (stage != FFN_BWD_WEIGHTS) return DSALT_OK;
-  // no tokens: the weight gradients are 0
-  const size_t es = p->w_grad_f32 ? 4 : 2;
-  cudaError_t e = cudaSuccess;
-  if (p->dw_gate) e = cudaMemsetAsync(p->dw_gate, 0, (size_t)p->F * p->d * es, st);
-  if (e == cudaSuccess && p->dw_up) e = cudaMemsetAsync(p->dw_up, 0, (size_t)p->F * p->d * es, st);
-  if (e == cudaSuccess && p->dw_down) e = cudaMemsetAsync(p->dw_down, 0, (size_t)p->d_out * p->F * es, st);
+  if (ffn_few_tokens(*p)) return status_of(launch_ffn_few(*p, st));
+  cudaError_t e = launch_ffn_tc(FFN_HIDDEN, *p, st);
+  if (e == cudaSuccess) e = launch_ffn_tc(FFN_OUT, *p, st);
   return status_of(e);
 }
 
-int dsalt_gated_ffn_hidden(const DsaltGatedFfnParams* p, void* stream) { return run_ffn(p, FFN_HIDDEN, stream); }
-int dsalt_gated_ffn_out(const DsaltGatedFfnParams* p, void* stream) { return run_ffn(p, FFN_OUT, stream); }
-int dsalt_gated_ffn_bwd_hidden(const DsaltGatedFfnParams* p, void* stream) { return run_ffn(p, FFN_BWD_HIDDEN, stream); }
-int dsalt_gated_ffn_bwd_input(const DsaltGatedFfnParams* p, void* stream) { return run_ffn(p, FFN_BWD_INPUT, stream); }
-int dsalt_gated_ffn_bwd_weights(const DsaltGatedFfnParams* p, void* stream) { return run_ffn(p, FFN_BWD_WEIGHTS, stream); }
+int dsalt_gated_ffn_bwd(const DsaltGatedFfnParams* p, void* stream) {
+  const int rc = check_ffn(p, true);
+  if (rc != DSALT_OK) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t e = cudaSuccess;
+  if (p->T == 0) {  // no tokens: the weight gradients are 0
+    const size_t es = p->w_grad_f32 ? 4 : 2;
+    if (p->dw_gate) e = cudaMemsetAsync(p->dw_gate, 0, (size_t)p->F * p->d * es, st);
+    if (e == cudaSuccess && p->dw_up) e = cudaMemsetAsync(p->dw_up, 0, (size_t)p->F * p->d * es, st);
+    if (e == cudaSuccess && p->dw_down) e = cudaMemsetAsync(p->dw_down, 0, (size_t)p->d_out * p->F * es, st);
+    return status_of(e);
+  }
+  if (p->dx || p->dw_gate || p->dw_up) e = launch_ffn_tc(FFN_BWD_HIDDEN, *p, st);
+  if (e == cudaSuccess && p->dx) e = launch_ffn_tc(FFN_BWD_INPUT, *p, st);
+  if (e == cudaSuccess) e = launch_ffn_tc(FFN_BWD_WEIGHTS, *p, st);
+  return status_of(e);
+}
 
 int dsalt_dropout(const DsaltDropoutParams* p, void* stream) {
   if (!p || p->n < 0 || p->threshold < 0 || p->threshold > 65536) return DSALT_ERR_ARG;

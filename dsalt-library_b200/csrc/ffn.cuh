@@ -1,9 +1,13 @@
-// Stages of the gated feed-forward block (ffn_tc.cu), in the order a training step runs them.
+// Stages of the gated feed-forward block, in the order a training step runs them.
 #pragma once
 
 #include "common.cuh"
 
 namespace dsalt {
 enum FfnStage { FFN_HIDDEN = 0, FFN_OUT = 1, FFN_BWD_HIDDEN = 2, FFN_BWD_INPUT = 3, FFN_BWD_WEIGHTS = 4 };
-cudaError_t launch_ffn(int stage, const DsaltGatedFfnParams& p, cudaStream_t st);
+// any number of tokens, tensor cores (ffn_tc.cu)
+cudaError_t launch_ffn_tc(int stage, const DsaltGatedFfnParams& p, cudaStream_t st);
+// the forward for few tokens (ffn_few.cu): both stages, the second launched early
+bool ffn_few_tokens(const DsaltGatedFfnParams& p);
+cudaError_t launch_ffn_few(const DsaltGatedFfnParams& p, cudaStream_t st);
 }  // namespace dsalt

@@ -25,7 +25,7 @@
 //   warp 0      TMA loads of this CTA's halves (128-byte swizzle); the leader's FULL
 //               barrier counts both CTAs' bytes
 //   warp 1      TMEM owner; in the leader the single-thread MMA issuer
-//   warps 2-17  epilogue: TMEM lane quadrant warp % 4, every fourth 32-column chunk;
+//   warps 2-…   epilogue: TMEM lane quadrant warp % 4, 32-column chunks in turn;
 //               a lane owns a row, so results are staged in shared memory and copied
 //               with row-contiguous 16-byte accesses (TMA stores of the same 64-byte
 //               rows shared the TMA unit with the operands' loads: hidden 175 us
@@ -36,15 +36,13 @@
 #include <initializer_list>
 
 #include "ffn.cuh"
-#include "tc_pair.cuh"
+#include "ffn_act.cuh"
 
 namespace dsalt {
 namespace ffn {
 
 constexpr int BM = 256, BK = 64;
 constexpr int kPiece = 128 * BK * 2;       // 128 rows (or columns) × 64 K of one operand
-constexpr int kEpiWarps = 16;
-constexpr int kThreads = (2 + kEpiWarps) * 32;
 constexpr int kBox = 2048;                 // staged box: 32 rows × 64 bytes
 constexpr int kMaxProb = 3;
 enum Epi { EPI_STORE = 0, EPI_HIDDEN = 1, EPI_DHIDDEN = 2 };
@@ -52,8 +50,14 @@ enum Epi { EPI_STORE = 0, EPI_HIDDEN = 1, EPI_DHIDDEN = 2 };
 template <int BN, int EPI>
 struct Cfg {
   static constexpr int kStageBytes = kPiece + BN / 2 * BK * 2;  // A's and B's halves of this CTA
+  // dhidden reads three boxes a chunk from memory: twice the warps keep enough of them on
+  // the way (115 us; 129 with 8 warps and a fifth stage).  The others take the stage that
+  // the smaller staging leaves (hidden 158 us; 166 with 16 warps and 5 stages).
+  static constexpr int kEpiWarps = EPI == EPI_DHIDDEN ? 16 : 8;
+  static constexpr int kThreads = (2 + kEpiWarps) * 32;
+  static constexpr int kColStep = kEpiWarps / 4 * 32;           // columns from a warp's chunk to its next
   static constexpr int kBoxes = EPI == EPI_DHIDDEN ? 3 : 2;     // staged boxes of a warp
-  static constexpr int kStages = BN == 256 ? (EPI == EPI_DHIDDEN ? 4 : 5) : 6;
+  static constexpr int kStages = EPI == EPI_DHIDDEN ? 4 : 6;
   static constexpr int FULL = 0, EMPTY = kStages, ACC_FULL = 2 * kStages, ACC_EMPTY = ACC_FULL + 2,
                        FINAL = ACC_EMPTY + 2, NB = FINAL + 1;
   struct alignas(1024) Smem {
@@ -92,32 +96,6 @@ __device__ __forceinline__ Tile decode(const Args& a, int t) {
   r.m0 = (t - begin) / nt * BM;
   r.nt = (t - begin) % nt;
   return r;
-}
-
-// ---------------------------------------------------------------- activation
-// act(g) and act'(g).  exp and the reciprocal are the fast ones (relative error
-// below 2^-20 over the range where the result is not rounded to 0 or g): the
-// results are rounded to 16 or 24 bits next.
-template <int ACT>
-__device__ __forceinline__ void act_pair(float g, float& a, float& da) {
-  constexpr float kLog2e = 1.4426950409f;
-  if constexpr (ACT == DSALT_ACT_SILU) {
-    const float sig = sm100::fast_rcp(1.f + sm100::fast_exp2(-kLog2e * g));
-    a = g * sig;
-    da = fmaf(a, 1.f - sig, sig);
-  } else if constexpr (ACT == DSALT_ACT_GELU) {
-    const float cdf = normcdff(g);
-    a = g * cdf;
-    da = fmaf(g * 0.3989422804f, sm100::fast_exp2(-0.5f * kLog2e * g * g), cdf);
-  } else {
-    // ½(1 + tanh z) = σ(2z), ½(1 − tanh² z) = 2σ(1 − σ), z = √(2/π)(g + 0.044715 g³)
-    const float g2 = g * g;
-    const float z2 = 1.5957691216f * g * fmaf(0.044715f, g2, 1.f);
-    const float sig = sm100::fast_rcp(1.f + sm100::fast_exp2(-kLog2e * z2));
-    const float w = sig * (1.f - sig);
-    a = g * sig;
-    da = sig + (w > 0.f ? g * w * 1.5957691216f * fmaf(0.134145f, g2, 1.f) : 0.f);
-  }
 }
 
 // ------------------------------------------------------------------- staging
@@ -165,10 +143,6 @@ __device__ __forceinline__ void rows_to_box(uint32_t box, const uint16_t* in, in
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
-// bytes 2 and 3 of two words: the upper 16 bits of fp32 x (low half) and y
-__device__ __forceinline__ uint32_t upper16(float x, float y) {
-  return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
-}
 
 // ------------------------------------------------------------------- kernel
 // AMN / BMN: the operand's K is the strided dimension (MN-major) instead of the
@@ -190,7 +164,7 @@ __device__ __forceinline__ uint64_t piece_desc(uint32_t addr, int kk) {
 }
 
 template <bool AMN, bool BMN, int EPI, int BN, int ACT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) ffn_gemm_kernel(const __grid_constant__ Args a) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI>::kThreads, 1) ffn_gemm_kernel(const __grid_constant__ Args a) {
   using namespace sm100;
   using C = Cfg<BN, EPI>;
   constexpr int kStages = C::kStages;
@@ -206,7 +180,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) ffn_gem
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar[C::ACC_FULL + b], 1);
-      mbar_init(bar[C::ACC_EMPTY + b], 2 * kEpiWarps);
+      mbar_init(bar[C::ACC_EMPTY + b], 2 * C::kEpiWarps);
     }
     mbar_init(bar[C::FINAL], 1);
     fence_mbar_init();
@@ -310,8 +284,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) ffn_gem
         if (lane == 0) mbar_arrive_cluster(map_rank(bar[C::ACC_EMPTY + acc], 0));
       };
 #pragma unroll 1
-      for (int c = cg * 32; c < kCols; c += 128) {
-        const bool last = c + 128 >= kCols;
+      for (int c = cg * 32; c < kCols; c += C::kColStep) {
+        const bool last = c + C::kColStep >= kCols;
         if constexpr (EPI == EPI_HIDDEN) {
           uint32_t wh[16], wa[16], wb[16], wl[16];
 #pragma unroll
@@ -332,9 +306,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) ffn_gem
               wh[k] = pack2(u[j] * a0, u[j + 1] * a1, a.bf16);
               wa[k] = upper16(a0, a1);
               wb[k] = upper16(d0, d1);
-              // byte 1 of a0, d0, a1, d1
-              wl[k] = __byte_perm(__byte_perm(__float_as_uint(a0), __float_as_uint(d0), 0x0051),
-                                  __byte_perm(__float_as_uint(a1), __float_as_uint(d1), 0x0051), 0x5410);
+              wl[k] = next8(a0, d0, a1, d1);
             }
           }
           stage_words(box, lane, wh);
@@ -384,7 +356,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) ffn_gem
           box_to_rows(box, a.f[3] + at + c, a.ld_f, rows, cols - c);
           box_to_rows(box + kBox, a.f[4] + at + c, a.ld_f, rows, cols - c);
           __syncwarp();
-          if (c + 128 < kCols) load_ab(c + 128);
+          if (!last) load_ab(c + C::kColStep);
         } else {
           float v[32];
           tmem_ld32(tacc + c, v);
@@ -453,29 +425,67 @@ cudaError_t sm_count(int* out) {
   return cudaSuccess;
 }
 
-void add_problem(Args& a, int64_t M, int64_t N, int tile_n, void* out, int64_t ld_out) {
-  Problem& p = a.prob[a.n_prob];
-  p.M = (int)M;
-  p.N = (int)N;
-  p.m_tiles = (int)((M + BM - 1) / BM);
-  p.n_tiles = (int)((N + tile_n - 1) / tile_n);
-  p.out = out;
-  p.ld_out = ld_out;
-  a.n_tiles += p.m_tiles * p.n_tiles;
-  p.tile_end = a.n_tiles;
-  ++a.n_prob;
+// The products of one launch, before the tile width is chosen.
+struct Job { int64_t M, N; void* out; int64_t ld_out; };
+struct Jobs {
+  const Job* first;
+  int n;
+  const Job* begin() const { return first; }
+  const Job* end() const { return first + n; }
+};
+
+int tiles_of(const Jobs& jobs, int cols) {
+  int64_t n = 0;
+  for (const Job& j : jobs) n += (j.M + BM - 1) / BM * ((j.N + cols - 1) / cols);
+  return (int)n;
+}
+
+// Tile columns (B rows of a pair) by estimated time: waves of tiles over the pairs ×
+// (K steps × a step's cycles + start and epilogue).  BN_COMMENT
+int pick_bn(const Jobs& jobs, int steps, bool halves, bool b_mn, int pairs) {
+#ifdef FORCE_BN
+  return b_mn && FORCE_BN < 128 ? 128 : FORCE_BN;
+#endif
+  int best = 256;
+  int64_t best_cost = INT64_MAX;
+  for (const int bn : {256, 128, 64}) {
+    if (bn == 64 && b_mn) break;
+    const int64_t waves = (tiles_of(jobs, halves ? bn / 2 : bn) + pairs - 1) / pairs;
+    const int64_t cost = waves * ((int64_t)steps * (bn == 256 ? 640 : bn == 128 ? 400 : 300) + 2000);
+    if (cost < best_cost) best = bn, best_cost = cost;
+  }
+  return best;
+}
+
+void set_jobs(Args& a, const Jobs& jobs, int cols) {
+  for (const Job& j : jobs) {
+    Problem& p = a.prob[a.n_prob++];
+    p.M = (int)j.M;
+    p.N = (int)j.N;
+    p.m_tiles = (int)((j.M + BM - 1) / BM);
+    p.n_tiles = (int)((j.N + cols - 1) / cols);
+    p.out = j.out;
+    p.ld_out = j.ld_out;
+    a.n_tiles += p.m_tiles * p.n_tiles;
+    p.tile_end = a.n_tiles;
+  }
 }
 
 template <bool AMN, bool BMN, int EPI, int BN, int ACT = 0>
-cudaError_t launch(const Args& a, cudaStream_t st) {
+cudaError_t launch_bn(const Args& a, int pairs, cudaStream_t st) {
   auto kernel = ffn_gemm_kernel<AMN, BMN, EPI, BN, ACT>;
   const size_t smem = sizeof(typename Cfg<BN, EPI>::Smem) + 1024;
   cudaError_t e = ensure_smem((const void*)kernel, smem);
   if (e != cudaSuccess) return e;
-  int sms = 0;
-  if ((e = sm_count(&sms)) != cudaSuccess) return e;
-  kernel<<<(unsigned)(2 * std::min(a.n_tiles, sms / 2)), kThreads, smem, st>>>(a);
+  kernel<<<(unsigned)(2 * std::min(a.n_tiles, pairs)), Cfg<BN, EPI>::kThreads, smem, st>>>(a);
   return cudaGetLastError();
+}
+template <bool AMN, bool BMN, int EPI, int ACT = 0>
+cudaError_t launch(const Args& a, int bn, int pairs, cudaStream_t st) {
+  if (bn == 256) return launch_bn<AMN, BMN, EPI, 256, ACT>(a, pairs, st);
+  if constexpr (!BMN)
+    if (bn == 64) return launch_bn<AMN, BMN, EPI, 64, ACT>(a, pairs, st);
+  return launch_bn<AMN, BMN, EPI, 128, ACT>(a, pairs, st);
 }
 
 Args base_args(const DsaltGatedFfnParams& p) {
@@ -501,7 +511,7 @@ void set_out(Args& a, bool f32) {
 
 }  // namespace ffn
 
-cudaError_t launch_ffn(int stage, const DsaltGatedFfnParams& p, cudaStream_t st) {
+cudaError_t launch_ffn_tc(int stage, const DsaltGatedFfnParams& p, cudaStream_t st) {
   using namespace ffn;
   // the tensor maps need the device's context current on this thread, which a thread
   // that has only allocated (a backward's first call) need not have: setting the device does it
@@ -509,64 +519,87 @@ cudaError_t launch_ffn(int stage, const DsaltGatedFfnParams& p, cudaStream_t st)
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaSetDevice(dev);
   if (e != cudaSuccess) return e;
+  int sms = 0;
+  if ((e = sm_count(&sms)) != cudaSuccess) return e;
+  const int pairs = sms / 2;
   Args a = base_args(p);
   const int dt = p.dtype;
-  constexpr int BN = 256;
   const cudaError_t bad = cudaErrorInvalidValue;
+  auto steps = [](int64_t k) { return (int)((k + BK - 1) / BK); };
   switch (stage) {
-    case FFN_HIDDEN:
+    case FFN_HIDDEN: {
       a.K = p.d;
       a.keep = p.a != nullptr;
-      if (!encode(&a.ma[0], dt, p.x, p.T, p.d, p.ld_x, false, 128) ||
-          !encode(&a.mb[0], dt, p.w_gate, p.F, p.d, p.ld_wg, false, BN / 2) ||
-          !encode(&a.mb[1], dt, p.w_up, p.F, p.d, p.ld_wu, false, BN / 2))
-        return bad;
+      const Job job = {p.T, p.F, nullptr, 0};
+      const Jobs jobs = {&job, 1};
+      const int bn = pick_bn(jobs, steps(a.K), true, false, pairs);
+      set_jobs(a, jobs, bn / 2);
       set_f(a, {p.h, p.a, p.b, p.ab});
-      add_problem(a, p.T, p.F, BN / 2, nullptr, 0);
-      if (p.activation == DSALT_ACT_SILU) return launch<false, false, EPI_HIDDEN, BN, DSALT_ACT_SILU>(a, st);
-      if (p.activation == DSALT_ACT_GELU) return launch<false, false, EPI_HIDDEN, BN, DSALT_ACT_GELU>(a, st);
-      return launch<false, false, EPI_HIDDEN, BN, DSALT_ACT_GELU_TANH>(a, st);
-    case FFN_OUT:
-      a.K = p.F;
-      add_problem(a, p.T, p.d_out, BN, p.y, p.d_out);
-      if (!encode(&a.ma[0], dt, p.h, p.T, p.F, p.ld_f, false, 128) ||
-          !encode(&a.mb[0], dt, p.w_down, p.d_out, p.F, p.ld_wd, false, BN / 2))
+      if (!encode(&a.ma[0], dt, p.x, p.T, p.d, p.ld_x, false, 128) ||
+          !encode(&a.mb[0], dt, p.w_gate, p.F, p.d, p.ld_wg, false, bn / 2) ||
+          !encode(&a.mb[1], dt, p.w_up, p.F, p.d, p.ld_wu, false, bn / 2))
         return bad;
+      if (p.activation == DSALT_ACT_SILU) return launch<false, false, EPI_HIDDEN, DSALT_ACT_SILU>(a, bn, pairs, st);
+      if (p.activation == DSALT_ACT_GELU) return launch<false, false, EPI_HIDDEN, DSALT_ACT_GELU>(a, bn, pairs, st);
+      return launch<false, false, EPI_HIDDEN, DSALT_ACT_GELU_TANH>(a, bn, pairs, st);
+    }
+    case FFN_OUT: {
+      a.K = p.F;
+      const Job job = {p.T, p.d_out, p.y, p.d_out};
+      const Jobs jobs = {&job, 1};
+      const int bn = pick_bn(jobs, steps(a.K), false, false, pairs);
+      set_jobs(a, jobs, bn);
       set_out(a, false);
-      return launch<false, false, EPI_STORE, BN>(a, st);
-    case FFN_BWD_HIDDEN:
+      if (!encode(&a.ma[0], dt, p.h, p.T, p.F, p.ld_f, false, 128) ||
+          !encode(&a.mb[0], dt, p.w_down, p.d_out, p.F, p.ld_wd, false, bn / 2))
+        return bad;
+      return launch<false, false, EPI_STORE>(a, bn, pairs, st);
+    }
+    case FFN_BWD_HIDDEN: {
       a.K = p.d_out;
+      const Job job = {p.T, p.F, nullptr, 0};
+      const Jobs jobs = {&job, 1};
+      const int bn = pick_bn(jobs, steps(a.K), false, true, pairs);
+      set_jobs(a, jobs, bn);
+      set_f(a, {p.a, p.b, p.ab, p.du, p.dg});
       if (!encode(&a.ma[0], dt, p.dy, p.T, p.d_out, p.ld_dy, false, 128) ||
           !encode(&a.mb[0], dt, p.w_down, p.d_out, p.F, p.ld_wd, true, 0))
         return bad;
-      set_f(a, {p.a, p.b, p.ab, p.du, p.dg});
-      add_problem(a, p.T, p.F, BN, nullptr, 0);
-      return launch<false, true, EPI_DHIDDEN, BN>(a, st);
-    case FFN_BWD_INPUT:
+      return launch<false, true, EPI_DHIDDEN>(a, bn, pairs, st);
+    }
+    case FFN_BWD_INPUT: {
       a.K = p.F;
       a.n_seg = 2;
-      add_problem(a, p.T, p.d, BN, p.dx, p.d);
+      const Job job = {p.T, p.d, p.dx, p.d};
+      const Jobs jobs = {&job, 1};
+      const int bn = pick_bn(jobs, 2 * steps(a.K), false, true, pairs);
+      set_jobs(a, jobs, bn);
+      set_out(a, false);
       if (!encode(&a.ma[0], dt, p.dg, p.T, p.F, p.ld_f, false, 128) || !encode(&a.ma[1], dt, p.du, p.T, p.F, p.ld_f, false, 128) ||
           !encode(&a.mb[0], dt, p.w_gate, p.F, p.d, p.ld_wg, true, 0) || !encode(&a.mb[1], dt, p.w_up, p.F, p.d, p.ld_wu, true, 0))
         return bad;
-      set_out(a, false);
-      return launch<false, true, EPI_STORE, BN>(a, st);
+      return launch<false, true, EPI_STORE>(a, bn, pairs, st);
+    }
     case FFN_BWD_WEIGHTS: {
       a.K = (int)p.T;
-      struct { const void* l; int64_t nl, ldl; const void* r; int64_t nr, ldr; void* out; } job[3] = {
+      struct { const void* l; int64_t nl, ldl; const void* r; int64_t nr, ldr; void* out; } all[3] = {
           {p.dg, p.F, p.ld_f, p.x, p.d, p.ld_x, p.dw_gate},
           {p.du, p.F, p.ld_f, p.x, p.d, p.ld_x, p.dw_up},
           {p.dy, p.d_out, p.ld_dy, p.h, p.F, p.ld_f, p.dw_down}};
-      for (const auto& j : job) {
+      Job job[3];
+      int n = 0;
+      for (const auto& j : all) {
         if (!j.out) continue;
-        const int i = a.n_prob;
-        if (!encode(&a.ma[i], dt, j.l, p.T, j.nl, j.ldl, true, 0) || !encode(&a.mb[i], dt, j.r, p.T, j.nr, j.ldr, true, 0))
+        if (!encode(&a.ma[n], dt, j.l, p.T, j.nl, j.ldl, true, 0) || !encode(&a.mb[n], dt, j.r, p.T, j.nr, j.ldr, true, 0))
           return bad;
-        add_problem(a, j.nl, j.nr, BN, j.out, j.nr);
+        job[n++] = Job{j.nl, j.nr, j.out, j.nr};
       }
-      if (a.n_prob == 0) return cudaSuccess;
+      if (n == 0) return cudaSuccess;
+      const Jobs jobs = {job, n};
+      const int bn = pick_bn(jobs, steps(a.K), false, true, pairs);
+      set_jobs(a, jobs, bn);
       set_out(a, p.w_grad_f32 != 0);
-      return launch<true, true, EPI_STORE, BN>(a, st);
+      return launch<true, true, EPI_STORE>(a, bn, pairs, st);
     }
   }
   return bad;

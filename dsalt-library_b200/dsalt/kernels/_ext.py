@@ -193,11 +193,8 @@ _ENTRY = {
     "dsalt_swiglu_fwd": SwigluParams,
     "dsalt_swiglu_bwd": SwigluParams,
     "dsalt_gqa_reduce": GqaReduceParams,
-    "dsalt_gated_ffn_hidden": GatedFfnParams,
-    "dsalt_gated_ffn_out": GatedFfnParams,
-    "dsalt_gated_ffn_bwd_hidden": GatedFfnParams,
-    "dsalt_gated_ffn_bwd_input": GatedFfnParams,
-    "dsalt_gated_ffn_bwd_weights": GatedFfnParams,
+    "dsalt_gated_ffn_fwd": GatedFfnParams,
+    "dsalt_gated_ffn_bwd": GatedFfnParams,
     "dsalt_dropout": DropoutParams,
     "dsalt_residual_norm_fwd": ResidualNormParams,
     "dsalt_residual_norm_bwd": ResidualNormParams,
@@ -274,15 +271,12 @@ def call(name: str, params) -> None:
         rec.append((name, e0, e1))
 
 
-def call_on(device: torch.device, names, params) -> None:
-    """``call`` each of ``names`` with the same parameters on the current stream of
-    ``device``, which need not be the current device."""
-    if device.index is None or device.index == torch._C._cuda_getDevice():
-        for name in names:
-            call(name, params)
-        return
-    with torch.cuda.device(device):
-        for name in names:
+def call_on(device: torch.device, name: str, params) -> None:
+    """``call`` on the current stream of ``device``, which need not be the current device."""
+    if device.index == torch._C._cuda_getDevice():
+        call(name, params)
+    else:
+        with torch.cuda.device(device):
             call(name, params)
 
 

@@ -37,7 +37,7 @@ def _launch(x: torch.Tensor, seed: torch.Tensor, site: int, threshold: int) -> t
     y = torch.empty_like(x)
     p = _ext.DropoutParams(x=x.data_ptr(), y=y.data_ptr(), seed=seed.data_ptr(), n=x.numel(), site=site,
                            threshold=threshold, dtype=_ext.dtype_code(x.dtype))
-    _ext.call_on(x.device, ("dsalt_dropout",), p)
+    _ext.call_on(x.device, "dsalt_dropout", p)
     return y
 
 

@@ -56,7 +56,7 @@ def _forward(x2, wg, wu, wd, activation: int, dtype: torch.dtype, keep: bool):
     h, a, b, ab = (torch.empty(p.T, p.ld_f, dtype=dtype, device=dev) if i == 0 or keep else None for i in range(4))
     y = torch.empty(p.T, p.d_out, dtype=dtype, device=dev)
     p.h, p.a, p.b, p.ab, p.y = h.data_ptr(), _ext.ptr(a), _ext.ptr(b), _ext.ptr(ab), y.data_ptr()
-    _ext.call_on(dev, ("dsalt_gated_ffn_hidden", "dsalt_gated_ffn_out"), p)
+    _ext.call_on(dev, "dsalt_gated_ffn_fwd", p)
     return y, h, a, b, ab
 
 
@@ -82,16 +82,13 @@ class GatedFFNFunction(torch.autograd.Function):
         dy_, p.ld_dy = _operand(dy, dtype)
         need_x, *need_w = ctx.needs_input_grad[:4]
         p.h, p.a, p.b, p.ab, p.dy = h.data_ptr(), a.data_ptr(), b.data_ptr(), ab.data_ptr(), dy_.data_ptr()
-        stages = []
         if need_x or need_w[0] or need_w[1]:
             dg, du = torch.empty_like(a), torch.empty_like(a)
             p.dg, p.du = dg.data_ptr(), du.data_ptr()
-            stages.append("dsalt_gated_ffn_bwd_hidden")
         grads = [None] * 4
         if need_x:
             grads[0] = torch.empty(p.T, p.d, dtype=dtype, device=dev)
             p.dx = grads[0].data_ptr()
-            stages.append("dsalt_gated_ffn_bwd_input")
         if any(need_w):
             # fp32 sums where a weight is not of the compute dtype: its gradient is rounded once
             p.w_grad_f32 = int(any(dt != dtype for dt in ctx.dtypes[1:]))
@@ -101,8 +98,7 @@ class GatedFFNFunction(torch.autograd.Function):
                 if need:
                     grads[1 + i] = torch.empty(shape, dtype=out, device=dev)
             p.dw_gate, p.dw_up, p.dw_down = (_ext.ptr(t) for t in grads[1:])
-            stages.append("dsalt_gated_ffn_bwd_weights")
-        _ext.call_on(dev, stages, p)
+        _ext.call_on(dev, "dsalt_gated_ffn_bwd", p)
         return (*(t if t is None else t.to(dt) for t, dt in zip(grads, ctx.dtypes)), None, None)
 
 

@@ -39,7 +39,7 @@ def _forward(x, f, gate, vectors, f32, seed, eps, site, threshold, gate_mode, ke
     rf = torch.empty(p.T, dtype=torch.float32, device=f.device) if keep and post is not None else None
     r = torch.empty(p.T, dtype=torch.float32, device=f.device) if keep and norm is not None else None
     p.x, p.h, p.rf, p.r = x.data_ptr(), _ext.ptr(h), _ext.ptr(rf), _ext.ptr(r)
-    _ext.call_on(f.device, ("dsalt_residual_norm_fwd",), p)
+    _ext.call_on(f.device, "dsalt_residual_norm_fwd", p)
     return x_new, h, rf, r
 
 
@@ -79,7 +79,7 @@ class ResidualNormFunction(torch.autograd.Function):
         p.rf, p.r, p.dx_new, p.dh = _ext.ptr(rf), _ext.ptr(r), _ext.ptr(dx_new), _ext.ptr(dh)
         p.dx, p.df, p.dgate, p.parts = dx.data_ptr(), df.data_ptr(), _ext.ptr(dgate), parts.data_ptr()
         p.dpost, p.dscale, p.dnorm = _ext.ptr(dpost), _ext.ptr(dscale), _ext.ptr(dnorm)
-        _ext.call_on(f.device, ("dsalt_residual_norm_bwd",), p)
+        _ext.call_on(f.device, "dsalt_residual_norm_bwd", p)
         dpost, dscale, dnorm = (t if t is None else t.to(dt) for t, dt in zip((dpost, dscale, dnorm), ctx.dtypes))
         return dx, df, dpost, dscale, dgate, dnorm, None, None, None, None, None
 

@@ -493,19 +493,17 @@ DSALT_API int dsalt_swiglu_bwd(const DsaltSwigluParams* p, void* stream);
 
 /* Gated feed-forward block, f16 / bf16, fp32 accumulation:
  *   g = x·Wgᵀ, u = x·Wuᵀ, h = act(g)⊙u, y = h·Wdᵀ
- * (dsalt/modules/dsalt_transformer.py:10-21 with act = silu), as five stages that
- * read their operands in place (row-major, row strides ld_*):
- *   hidden       h, rounded once from fp32, and for a later backward a = act(g) and
- *                b = u⊙act'(g) as the upper 24 bits of their fp32 values: the upper 16
- *                in a and b, the next 8 of each in the low and high byte of ab (all
- *                three or none); g and u are not stored
- *   out          y
- *   bwd_hidden   dh = dy·Wd (kept in fp32), du = R(dh⊙a), dg = R(dh⊙b)
- *   bwd_input    dx = R(dg·Wg + du·Wu), one accumulation
- *   bwd_weights  dWg = dgᵀ·x, dWu = duᵀ·x, dWd = dyᵀ·h, those whose pointer is set,
- *                in dtype, or in fp32 with w_grad_f32
- * Inputs and the stride ld_f of h, a, b, dg, du: 16-byte aligned, strides multiples
- * of 8.  y, dx and the weight gradients are dense, of any alignment.         */
+ * (dsalt/modules/dsalt_transformer.py:10-21 with act = silu).  Operands are row-major
+ * with row strides ld_* and read in place.  The forward writes y, h (rounded once from
+ * fp32) and, with a, b and ab set, what a backward needs of g and u: a = act(g) and
+ * b = u⊙act'(g) as the upper 24 bits of their fp32 values, the upper 16 in a and b,
+ * the next 8 of each in the low and high byte of ab.  The backward forms, of
+ *   dh = dy·Wd (kept in fp32), du = R(dh⊙a), dg = R(dh⊙b), dx = R(dg·Wg + du·Wu),
+ *   dWg = dgᵀ·x, dWu = duᵀ·x, dWd = dyᵀ·h,
+ * what the set ones of dx, dw_gate, dw_up and dw_down need; the weight gradients in
+ * dtype, or in fp32 with w_grad_f32.  Inputs and h, a, b, ab, dg, du: 16-byte aligned,
+ * strides multiples of 8; in those five columns F up to the next multiple of 8 may be
+ * written.  y, dx and the weight gradients are dense, of any alignment.      */
 enum { DSALT_ACT_SILU = 0, DSALT_ACT_GELU = 1, DSALT_ACT_GELU_TANH = 2 };
 typedef struct DsaltGatedFfnParams {
   const void* x;              /* [T, d] stride ld_x */
@@ -532,11 +530,8 @@ typedef struct DsaltGatedFfnParams {
   int32_t dtype;
   int32_t w_grad_f32;
 } DsaltGatedFfnParams;
-DSALT_API int dsalt_gated_ffn_hidden(const DsaltGatedFfnParams* p, void* stream);
-DSALT_API int dsalt_gated_ffn_out(const DsaltGatedFfnParams* p, void* stream);
-DSALT_API int dsalt_gated_ffn_bwd_hidden(const DsaltGatedFfnParams* p, void* stream);
-DSALT_API int dsalt_gated_ffn_bwd_input(const DsaltGatedFfnParams* p, void* stream);
-DSALT_API int dsalt_gated_ffn_bwd_weights(const DsaltGatedFfnParams* p, void* stream);
+DSALT_API int dsalt_gated_ffn_fwd(const DsaltGatedFfnParams* p, void* stream);
+DSALT_API int dsalt_gated_ffn_bwd(const DsaltGatedFfnParams* p, void* stream);
 
 /* Dropout without a stored mask, f16 / bf16 / f32.  Element i (row-major index) is
  * dropped when its 16-bit draw is below `threshold` = round(p·65536); kept elements

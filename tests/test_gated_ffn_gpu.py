@@ -261,8 +261,8 @@ def test_results_end_where_the_tensors_end():
                             y=P(y), dy=P(dy), dg=P(f[3]), du=P(f[4]), dx=P(dx), dw_gate=P(dws[0]), dw_up=P(dws[1]),
                             dw_down=P(dws[2]), T=T, ld_x=d, ld_wg=d, ld_wu=d, ld_wd=F, ld_f=80, ld_dy=d, d=d, F=F,
                             d_out=d, dtype=_ext.BF16, w_grad_f32=1)
-    for name in ("hidden", "out", "bwd_hidden", "bwd_input", "bwd_weights"):
-        _ext.call("dsalt_gated_ffn_" + name, p)
+    for name in ("dsalt_gated_ffn_fwd", "dsalt_gated_ffn_bwd"):
+        _ext.call(name, p)
     for t, n in [(t, T) for t in (*f, y, dx)] + list(zip(dws, (F, F, d))):
         assert (t[n:] == mark).all()
         assert not (t[:n, :min(F, t.shape[1])] == mark).all()
