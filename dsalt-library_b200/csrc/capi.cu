@@ -439,8 +439,8 @@ int dsalt_gated_ffn_fwd(const DsaltGatedFfnParams* p, void* stream) {
   if (rc != DSALT_OK || p->T == 0) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   if (ffn_few_tokens(*p)) return status_of(launch_ffn_few(*p, st));
-  cudaError_t e = launch_ffn_tc(FFN_HIDDEN, *p, st);
-  if (e == cudaSuccess) e = launch_ffn_tc(FFN_OUT, *p, st);
+  cudaError_t e = launch_ffn_tc(FFN_HIDDEN, *p, false, st);
+  if (e == cudaSuccess) e = launch_ffn_tc(FFN_OUT, *p, true, st);
   return status_of(e);
 }
 
@@ -456,9 +456,10 @@ int dsalt_gated_ffn_bwd(const DsaltGatedFfnParams* p, void* stream) {
     if (e == cudaSuccess && p->dw_down) e = cudaMemsetAsync(p->dw_down, 0, (size_t)p->d_out * p->F * es, st);
     return status_of(e);
   }
-  if (p->dx || p->dw_gate || p->dw_up) e = launch_ffn_tc(FFN_BWD_HIDDEN, *p, st);
-  if (e == cudaSuccess && p->dx) e = launch_ffn_tc(FFN_BWD_INPUT, *p, st);
-  if (e == cudaSuccess) e = launch_ffn_tc(FFN_BWD_WEIGHTS, *p, st);
+  const bool hidden = p->dx || p->dw_gate || p->dw_up;
+  if (hidden) e = launch_ffn_tc(FFN_BWD_HIDDEN, *p, false, st);
+  if (e == cudaSuccess && p->dx) e = launch_ffn_tc(FFN_BWD_INPUT, *p, true, st);
+  if (e == cudaSuccess) e = launch_ffn_tc(FFN_BWD_WEIGHTS, *p, hidden, st);
   return status_of(e);
 }
 

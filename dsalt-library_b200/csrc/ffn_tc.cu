@@ -30,7 +30,9 @@
 //               with row-contiguous 16-byte accesses (TMA stores of the same 64-byte
 //               rows shared the TMA unit with the operands' loads: hidden 175 us
 //               instead of HIDDEN_US at T = 16384, d = 1024, F = 2816)
-// Every wait is bounded (sm100::mbar_wait).
+// Every wait is bounded (sm100::mbar_wait).  Launches after the first of a call are
+// programmatic dependents: they set up their barriers and TMEM beside the end of the
+// launch before, and wait for its completion before they touch memory.
 #include <algorithm>
 #include <cstring>
 #include <initializer_list>
@@ -81,6 +83,7 @@ struct alignas(64) Args {
   Problem prob[kMaxProb];
   int n_prob, n_seg, K, n_tiles;
   bool bf16, out_f32, out_vec, keep;
+  bool early;      // launched beside its predecessor in the stream, one of these kernels
   uint16_t* f[5];  // [T, F] stride ld_f: hidden writes h, a, b, ab; dhidden reads a, b, ab, writes du, dg
   int64_t ld_f;
   int32_t* status;
@@ -173,6 +176,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI>::kThrea
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
   const BarArray bar{smem_u32(&sm.bars[0])};
+  // the next launch may set itself up beside this one; it waits for this one's results
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (tid == 64) {
+    for (int i = 0; i < kMaxProb; ++i) {
+      if (i > 0 && i >= a.n_prob && i >= a.n_seg && !(EPI == EPI_HIDDEN && i == 1)) break;
+      if (i == 0 || EPI != EPI_HIDDEN) prefetch_tmap(&a.ma[i]);
+      prefetch_tmap(&a.mb[i]);
+    }
+  }
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar[C::FULL + s], 1);
@@ -190,6 +202,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI>::kThrea
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // both CTAs' barriers exist before either signals the other's
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the launch before has written its results
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
   volatile int* abort_flag = &sm.abort_flag;
@@ -477,8 +490,17 @@ cudaError_t launch_bn(const Args& a, int pairs, cudaStream_t st) {
   const size_t smem = sizeof(typename Cfg<BN, EPI>::Smem) + 1024;
   cudaError_t e = ensure_smem((const void*)kernel, smem);
   if (e != cudaSuccess) return e;
-  kernel<<<(unsigned)(2 * std::min(a.n_tiles, pairs)), Cfg<BN, EPI>::kThreads, smem, st>>>(a);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * std::min(a.n_tiles, pairs)));
+  cfg.blockDim = dim3(Cfg<BN, EPI>::kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 template <bool AMN, bool BMN, int EPI, int ACT = 0>
 cudaError_t launch(const Args& a, int bn, int pairs, cudaStream_t st) {
@@ -511,7 +533,7 @@ void set_out(Args& a, bool f32) {
 
 }  // namespace ffn
 
-cudaError_t launch_ffn_tc(int stage, const DsaltGatedFfnParams& p, cudaStream_t st) {
+cudaError_t launch_ffn_tc(int stage, const DsaltGatedFfnParams& p, bool early, cudaStream_t st) {
   using namespace ffn;
   // the tensor maps need the device's context current on this thread, which a thread
   // that has only allocated (a backward's first call) need not have: setting the device does it
@@ -523,6 +545,7 @@ cudaError_t launch_ffn_tc(int stage, const DsaltGatedFfnParams& p, cudaStream_t 
   if ((e = sm_count(&sms)) != cudaSuccess) return e;
   const int pairs = sms / 2;
   Args a = base_args(p);
+  a.early = early;
   const int dt = p.dtype;
   const cudaError_t bad = cudaErrorInvalidValue;
   auto steps = [](int64_t k) { return (int)((k + BK - 1) / BK); };
