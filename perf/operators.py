@@ -264,9 +264,8 @@ def _plain_dropout(case, s):
 
 # ------------------------------------------------------- the framework's calls
 def _package():
-    root = str(Path(__file__).resolve().parents[1] / "dsalt-library_b200")
-    if root not in sys.path:
-        sys.path.insert(0, root)
+    if "dsalt" not in sys.modules:  # once: a user's program has imported the package
+        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "dsalt-library_b200"))
 
 
 def _own_ffn(case, s):
