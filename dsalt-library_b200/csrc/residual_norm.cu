@@ -11,10 +11,15 @@
 // once in and once out.
 //
 // A row belongs to a group of threads of eight consecutive columns each: 8, 16 or
-// 32 lanes of a warp up to d = 256, else a whole CTA of ceil(d / 256) warps (two
-// chunks of columns a thread past d = 8192).  A group walks rows of the grid's
-// stride, its weights and column sums in registers; the sums of a group go to one
-// partial row and a second kernel adds the partial rows in order.
+// 32 lanes of a warp up to d = 256, else a whole CTA (of one, two or four chunks of
+// columns a thread past d = 4096).  A group walks rows of the grid's stride with the
+// next row's loads on their way, its weights and column sums in registers; the sums of
+// a group go to one partial row and a second kernel adds the partial rows in order.
+//
+// The backward needs Σ dh⊙norm⊙x' before G, and Σ κ⊙G with κ = D⊙scale⊙gate⊙post⊙f
+// (for df and a token's dgate; κ there without the token's gate) after it.  G = u − e·x' with u = dx_new + r·dh⊙norm and
+// e = r³·mean(dh⊙norm⊙x') is linear in that first sum, so Σ κ⊙G = Σ κ⊙u − e·Σ κ⊙x':
+// one round of three sums a row instead of two dependent rounds.
 #include "dropout.cuh"
 
 namespace dsalt {
@@ -32,237 +37,290 @@ inline Shape shape_of(int d) {
   if (units <= 8) return {8, kSmallThreads, 1};
   if (units <= 16) return {16, kSmallThreads, 1};
   if (units <= 32) return {32, kSmallThreads, 1};
-  const int chunks = units <= 1024 ? 1 : 2;
+  const int chunks = units <= 512 ? 1 : units <= 1024 ? 2 : 4;
   const int t = ((units + chunks - 1) / chunks + 31) / 32 * 32;
   return {t, t, chunks};
 }
 
-// Sums over the row group: NV values at once; every thread gets the totals.
+// Eight consecutive elements of a row as they lie in memory, so that the next row's
+// can be on their way in few registers.
+template <typename T, bool VEC>
+struct Raw {
+  T e[8];
+  __device__ __forceinline__ void load(const T* p, int n) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = j < n ? p[j] : from_f32<T>(0.f);
+  }
+  __device__ __forceinline__ void zero() { load(nullptr, 0); }
+  __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(e[j]);
+  }
+};
+template <typename T>
+struct Raw<T, true> {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p, int) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void get(float* v) const {
+    const T* e = reinterpret_cast<const T*>(u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(e[j]);
+  }
+};
+
+// Sums over the row group, NV values at once; every thread gets the totals.  `red`: one
+// of two halves that calls use in turn, so that a call needs one barrier: a half is
+// written again only after the barrier of the call between.
 template <int NV>
 __device__ __forceinline__ void group_sum(float (&v)[NV], int group, float* red) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
-    for (int o = min(group, 32) / 2; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < group)
+#pragma unroll
+      for (int k = 0; k < NV; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
   if (group <= 32) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = group >> 5;
-  __syncthreads();  // the previous totals are read
   if (lane == 0)
 #pragma unroll
     for (int k = 0; k < NV; ++k) red[warp * NV + k] = v[k];
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    float s = lane < nw ? red[lane * NV + k] : 0.f;
-    v[k] = warp_sum(s);
-  }
+  for (int k = 0; k < NV; ++k) v[k] = 0.f;
+  for (int w = 0; w < nw; ++w)
+#pragma unroll
+    for (int k = 0; k < NV; ++k) v[k] += red[w * NV + k];
 }
 
 template <typename T>
 __device__ __forceinline__ void load_weights(const void* w, bool f32, int c, int d, float* v) {
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    v[j] = c + j < d ? (f32 ? __ldg(reinterpret_cast<const float*>(w) + c + j)
-                            : to_f32<T>(reinterpret_cast<const T*>(w)[c + j]))
-                     : 0.f;
+    v[j] = w && c + j < d ? (f32 ? __ldg(reinterpret_cast<const float*>(w) + c + j)
+                                 : to_f32<T>(reinterpret_cast<const T*>(w)[c + j]))
+                          : 1.f;
 }
 
-template <typename T, int CH, bool VEC>
-__global__ void __launch_bounds__(1024) residual_fwd_kernel(const DsaltResidualNormParams p, int group) {
-  __shared__ float red[32];
-  const int gid = threadIdx.x / group, lane = threadIdx.x - gid * group;
-  const int64_t groups = (int64_t)gridDim.x * (blockDim.x / group);
-  const int64_t first = (int64_t)blockIdx.x * (blockDim.x / group) + gid;
+constexpr int kMaxWarps = 16;
+
+template <typename T, int CH, bool VEC, int MAXT>
+__global__ void __launch_bounds__(MAXT) residual_fwd_kernel(const DsaltResidualNormParams p, int group) {
+  __shared__ float red[2][kMaxWarps];
+  const int gid = threadIdx.x / group, lane = threadIdx.x - gid * group, per_cta = blockDim.x / group;
+  const int64_t stride = (int64_t)gridDim.x * per_cta;
+  // every group of a CTA makes the same number of rounds (the sums synchronise)
+  const int64_t rounds = (p.T - (int64_t)blockIdx.x * per_cta + stride - 1) / stride;
   Dropout dr;
   dr.init(p.seed, p.site, p.threshold);
   const T* X = reinterpret_cast<const T*>(p.x);
   const T* Fv = reinterpret_cast<const T*>(p.f);
   const T* Gt = reinterpret_cast<const T*>(p.gate);
-  // every group of a CTA makes the same number of rounds (the sums synchronise)
-  const int64_t rounds = (p.T - (int64_t)blockIdx.x * (blockDim.x / group) + groups - 1) / groups;
-  for (int64_t k = 0; k < rounds; ++k) {
-    const int64_t t = first + k * groups;
-    const bool on = t < p.T;
-    float f[CH][8], x[CH][8];
-    float s[1] = {0.f};
+  const float inv_d = 1.f / (float)p.d;
+  // post·scale and norm of this thread's columns
+  float ws[CH][8], wn[CH][8];
+#pragma unroll
+  for (int ch = 0; ch < CH; ++ch) {
+    const int c = (lane + ch * group) * 8;
+    float w[8];
+    load_weights<T>(p.post, p.w_f32, c, p.d, w);
+    load_weights<T>(p.scale, p.w_f32, c, p.d, ws[ch]);
+    load_weights<T>(p.norm, p.w_f32, c, p.d, wn[ch]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ws[ch][j] *= w[j];
+  }
+  Raw<T, VEC> nx[CH], nf[CH];
+  auto fetch = [&](int64_t t) {
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (lane + ch * group) * 8;
-      const bool in = on && c < p.d;
+      if (t < p.T && c < p.d) {
+        nx[ch].load(X + t * p.d + c, p.d - c);
+        nf[ch].load(Fv + t * p.d + c, p.d - c);
+      } else {
+        nx[ch].zero();
+        nf[ch].zero();
+      }
+    }
+  };
+  int64_t t = (int64_t)blockIdx.x * per_cta + gid;
+  fetch(t);
+  for (int64_t k = 0; k < rounds; ++k, t += stride) {
+    const bool on = t < p.T;
+    float f[CH][8], x[CH][8], s[1] = {0.f};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[ch][j] = x[ch][j] = 0.f;
-      if (!in) continue;
-      load8<T, VEC>(Fv + t * p.d + c, p.d - c, f[ch]);
-      load8<T, VEC>(X + t * p.d + c, p.d - c, x[ch]);
+    for (int ch = 0; ch < CH; ++ch) {
+      nf[ch].get(f[ch]);
+      nx[ch].get(x[ch]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[0] = fmaf(f[ch][j], f[ch][j], s[0]);
     }
+    if (k + 1 < rounds) fetch(t + stride);
     float rf = 1.f;
     if (p.post) {
-      group_sum(s, group, red);
-      rf = rsqrtf(s[0] / (float)p.d + p.eps);
+      group_sum(s, group, red[0]);
+      rf = rsqrtf(fmaf(s[0], inv_d, p.eps));
       if (on && lane == 0 && p.rf) p.rf[t] = rf;
     }
-    const float gt = p.gate_mode == DSALT_GATE_TOKEN && on ? to_f32<T>(Gt[t]) : 1.f;
+    if (p.gate_mode == DSALT_GATE_TOKEN && on) rf *= to_f32<T>(Gt[t]);
     s[0] = 0.f;
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (lane + ch * group) * 8;
       if (!(on && c < p.d)) continue;
-      float w[8];
-      if (p.post) {
-        load_weights<T>(p.post, p.w_f32, c, p.d, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[ch][j] = f[ch][j] * rf * w[j];
-      }
-      if (p.scale) {
-        load_weights<T>(p.scale, p.w_f32, c, p.d, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[ch][j] *= w[j];
-      }
+      const int64_t at = t * p.d + c;
       if (p.gate_mode == DSALT_GATE_FULL) {
-        load8<T, VEC>(Gt + t * p.d + c, p.d - c, w);
+        float w[8];
+        load8<T, VEC>(Gt + at, p.d - c, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[ch][j] *= w[j];
-      } else if (p.gate_mode == DSALT_GATE_TOKEN) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[ch][j] *= gt;
       }
-      const uint32_t keep = p.threshold > 0 ? dr.keep8((uint64_t)(t * p.d + c)) : 0xffu;
+      const uint32_t keep = p.threshold > 0 ? (VEC ? dr.keep_block((uint64_t)at >> 3) : dr.keep8((uint64_t)at)) : 0xffu;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        x[ch][j] = round_to<T>((keep >> j & 1u) ? fmaf(f[ch][j], dr.scale, x[ch][j]) : x[ch][j]);
+        const float a = f[ch][j] * (ws[ch][j] * rf);
+        x[ch][j] = round_to<T>((keep >> j & 1u) ? fmaf(a, dr.scale, x[ch][j]) : x[ch][j]);
         s[0] = fmaf(x[ch][j], x[ch][j], s[0]);
       }
-      store8<T, VEC>(reinterpret_cast<T*>(p.x_new) + t * p.d + c, p.d - c, x[ch]);
+      store8<T, VEC>(reinterpret_cast<T*>(p.x_new) + at, p.d - c, x[ch]);
     }
     if (p.norm) {
-      group_sum(s, group, red);
-      const float r = rsqrtf(s[0] / (float)p.d + p.eps);
+      group_sum(s, group, red[1]);
+      const float r = rsqrtf(fmaf(s[0], inv_d, p.eps));
       if (on && lane == 0 && p.r) p.r[t] = r;
 #pragma unroll
       for (int ch = 0; ch < CH; ++ch) {
         const int c = (lane + ch * group) * 8;
         if (!(on && c < p.d)) continue;
-        float w[8];
-        load_weights<T>(p.norm, p.w_f32, c, p.d, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = x[ch][j] * r * w[j];
-        store8<T, VEC>(reinterpret_cast<T*>(p.h) + t * p.d + c, p.d - c, w);
+        for (int j = 0; j < 8; ++j) x[ch][j] = x[ch][j] * r * wn[ch][j];
+        store8<T, VEC>(reinterpret_cast<T*>(p.h) + t * p.d + c, p.d - c, x[ch]);
       }
     }
+    // with one sum a row the halves still alternate row by row
+    if (!(p.post && p.norm) && group > 32) __syncthreads();
   }
 }
 
-template <typename T, int CH, bool VEC>
-__global__ void __launch_bounds__(1024) residual_bwd_kernel(const DsaltResidualNormParams p, int group) {
-  __shared__ float red[64];
-  const int gid = threadIdx.x / group, lane = threadIdx.x - gid * group;
-  const int64_t groups = (int64_t)gridDim.x * (blockDim.x / group);
-  const int64_t first = (int64_t)blockIdx.x * (blockDim.x / group) + gid;
+template <typename T, int CH, bool VEC, int MAXT>
+__global__ void __launch_bounds__(MAXT, 512 / MAXT) residual_bwd_kernel(const DsaltResidualNormParams p, int group) {
+  // one chunk a thread: its weights stay in registers and the next row's loads go out
+  // early; with more chunks the registers are left to the column sums
+  constexpr bool kHold = CH == 1;
+  __shared__ float red[2][3 * kMaxWarps];
+  const int gid = threadIdx.x / group, lane = threadIdx.x - gid * group, per_cta = blockDim.x / group;
+  const int64_t stride = (int64_t)gridDim.x * per_cta, first = (int64_t)blockIdx.x * per_cta + gid;
+  const int64_t rounds = (p.T - (int64_t)blockIdx.x * per_cta + stride - 1) / stride;
   Dropout dr;
   dr.init(p.seed, p.site, p.threshold);
-  const T* Fv = reinterpret_cast<const T*>(p.f);
-  const T* Xn = reinterpret_cast<const T*>(p.x_new);
   const T* Gt = reinterpret_cast<const T*>(p.gate);
-  const bool with_h = p.norm && p.dh;
-  float a_scale[CH][8], a_post[CH][8], a_norm[CH][8];
+  const bool with_h = p.norm && p.dh, sums = with_h || p.post || p.gate_mode == DSALT_GATE_TOKEN;
+  const float inv_d = 1.f / (float)p.d;
+  float hp[8], hs[8], hn[8], a_scale[CH][8], a_post[CH][8], a_norm[CH][8];
+  auto weights = [&](int c) {
+    load_weights<T>(p.post, p.w_f32, c, p.d, hp);
+    load_weights<T>(p.scale, p.w_f32, c, p.d, hs);
+    load_weights<T>(p.norm, p.w_f32, c, p.d, hn);
+  };
+  if (kHold) weights(lane * 8);
 #pragma unroll
   for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
     for (int j = 0; j < 8; ++j) a_scale[ch][j] = a_post[ch][j] = a_norm[ch][j] = 0.f;
-  const int64_t rounds = (p.T - (int64_t)blockIdx.x * (blockDim.x / group) + groups - 1) / groups;
-  for (int64_t k = 0; k < rounds; ++k) {
-    const int64_t t = first + k * groups;
+  Raw<T, VEC> nx[CH], nf[CH], nd[CH], nh[CH];  // x', f, dx_new, dh
+  float nr = 0.f, nrf = 1.f, ngt = 1.f;
+  auto fetch = [&](int64_t t) {
     const bool on = t < p.T;
-    float g[CH][8], x[CH][8];  // G in the end; x'
-    const float r = with_h && on ? __ldg(p.r + t) : 0.f;
-    const float rf = p.post && on ? __ldg(p.rf + t) : 1.f;
-    if (with_h) {
-      float s[1] = {0.f};
-#pragma unroll
-      for (int ch = 0; ch < CH; ++ch) {
-        const int c = (lane + ch * group) * 8;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[ch][j] = x[ch][j] = 0.f;
-        if (!(on && c < p.d)) continue;
-        float w[8];
-        load8<T, VEC>(Xn + t * p.d + c, p.d - c, x[ch]);
-        load8<T, VEC>(reinterpret_cast<const T*>(p.dh) + t * p.d + c, p.d - c, g[ch]);
-        load_weights<T>(p.norm, p.w_f32, c, p.d, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          a_norm[ch][j] = fmaf(g[ch][j], x[ch][j] * r, a_norm[ch][j]);
-          g[ch][j] *= w[j];
-          s[0] = fmaf(g[ch][j], x[ch][j], s[0]);
-        }
-      }
-      group_sum(s, group, red);
-      const float m = r * r * s[0] / (float)p.d;
-#pragma unroll
-      for (int ch = 0; ch < CH; ++ch)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[ch][j] = r * fmaf(-x[ch][j], m, g[ch][j]);
-    } else {
-#pragma unroll
-      for (int ch = 0; ch < CH; ++ch)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[ch][j] = 0.f;
-    }
-    const float gt = p.gate_mode == DSALT_GATE_TOKEN && on ? to_f32<T>(Gt[t]) : 1.f;
-    float f[CH][8];
-    float s[2] = {0.f, 0.f};  // Σ dn·post·f, Σ D(G)·scale·n
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (lane + ch * group) * 8;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[ch][j] = 0.f;
-      if (!(on && c < p.d)) continue;
+      const bool in = on && c < p.d;
       const int64_t at = t * p.d + c;
-      float w[8], post[8], gate[8], scale[8];
-      if (p.dx_new) {
-        load8<T, VEC>(reinterpret_cast<const T*>(p.dx_new) + at, p.d - c, w);
+      auto one = [&](Raw<T, VEC>& raw, const void* q) {
+        if (in && q) raw.load(reinterpret_cast<const T*>(q) + at, p.d - c);
+        else raw.zero();
+      };
+      one(nx[ch], with_h ? p.x_new : nullptr);
+      one(nh[ch], with_h ? p.dh : nullptr);
+      one(nf[ch], p.f);
+      one(nd[ch], p.dx_new);
+    }
+    nr = with_h && on ? __ldg(p.r + t) : 0.f;
+    nrf = p.post && on ? __ldg(p.rf + t) : 1.f;
+    ngt = p.gate_mode == DSALT_GATE_TOKEN && on ? to_f32<T>(Gt[t]) : 1.f;
+  };
+  int64_t t = first;
+  fetch(t);
+  for (int64_t k = 0; k < rounds; ++k, t += stride) {
+    const bool on = t < p.T;
+    const float r = nr, rf = nrf, gt = ngt;
+    float u[CH][8], x[CH][8], f[CH][8];
+    uint32_t keep[CH];
+    float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[ch][j] += w[j];
-      }
-      store8<T, VEC>(reinterpret_cast<T*>(p.dx) + at, p.d - c, g[ch]);
-      load8<T, VEC>(Fv + at, p.d - c, f[ch]);
-      if (p.post) load_weights<T>(p.post, p.w_f32, c, p.d, post);
-      if (p.scale) load_weights<T>(p.scale, p.w_f32, c, p.d, scale);
-      if (p.gate_mode == DSALT_GATE_FULL) load8<T, VEC>(Gt + at, p.d - c, gate);
-      const uint32_t keep = p.threshold > 0 ? dr.keep8((uint64_t)at) : 0xffu;
+    for (int ch = 0; ch < CH; ++ch) {
+      const int c = (lane + ch * group) * 8;
+      const int64_t at = t * p.d + c;
+      float dh[8], gate[8];
+      nx[ch].get(x[ch]);
+      nf[ch].get(f[ch]);
+      nd[ch].get(u[ch]);
+      nh[ch].get(dh);
+      if (!kHold) weights(c);
+      keep[ch] = p.threshold > 0 ? (VEC ? dr.keep_block((uint64_t)at >> 3) : dr.keep8((uint64_t)at)) : 0xffu;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) gate[j] = 1.f;
+      if (p.gate_mode == DSALT_GATE_FULL && on && c < p.d) load8<T, VEC>(Gt + at, p.d - c, gate);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
+        const float q = dh[j] * hn[j];
+        a_norm[ch][j] = fmaf(dh[j], x[ch][j] * r, a_norm[ch][j]);
+        s[0] = fmaf(q, x[ch][j], s[0]);
+        u[ch][j] = fmaf(r, q, u[ch][j]);
         // a dropped element passes nothing back, whatever f holds there
-        const bool kept = (keep >> j & 1u) && (VEC || c + j < p.d);
-        const float da = kept ? g[ch][j] * dr.scale : 0.f;
-        const float fr = f[ch][j] * rf;
-        const float n = p.post ? fr * post[j] : fr;
-        const float sc = p.scale ? scale[j] : 1.f;
-        const float ga = p.gate_mode == DSALT_GATE_FULL ? gate[j] : gt;
-        const float dn = da * sc * ga;
-        const float dgn = kept ? da * n : 0.f;
-        a_scale[ch][j] = fmaf(dgn, ga, a_scale[ch][j]);
-        if (kept) a_post[ch][j] = fmaf(dn, fr, a_post[ch][j]);
-        w[j] = dgn * sc;  // dgate of a full gate
-        g[ch][j] = p.post ? dn * post[j] : dn;
-        s[0] = fmaf(g[ch][j], f[ch][j], s[0]);
-        s[1] += w[j];
+        const float kf = (keep[ch] >> j & 1u) ? f[ch][j] * hp[j] * (dr.scale * hs[j]) * gate[j] : 0.f;
+        s[1] = fmaf(kf, u[ch][j], s[1]);
+        s[2] = fmaf(kf, x[ch][j], s[2]);
       }
-      if (p.gate_mode == DSALT_GATE_FULL) store8<T, VEC>(reinterpret_cast<T*>(p.dgate) + at, p.d - c, w);
     }
-    if (p.post || p.gate_mode == DSALT_GATE_TOKEN) group_sum(s, group, red);
-    if (p.gate_mode == DSALT_GATE_TOKEN && on && lane == 0) reinterpret_cast<T*>(p.dgate)[t] = from_f32<T>(s[1]);
-    const float m = rf * rf * s[0] / (float)p.d;
+    if (kHold && k + 1 < rounds) fetch(t + stride);
+    if (sums) group_sum(s, group, red[k & 1]);
+    const float e = r * r * r * (s[0] * inv_d);
+    const float S = fmaf(-e, s[2], s[1]);  // Σ κ⊙G, without a token's gate
+    if (p.gate_mode == DSALT_GATE_TOKEN && on && lane == 0) reinterpret_cast<T*>(p.dgate)[t] = from_f32<T>(rf * S);
+    const float m = rf * rf * gt * (S * inv_d);
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (lane + ch * group) * 8;
       if (!(on && c < p.d)) continue;
-      if (p.post) {
+      const int64_t at = t * p.d + c;
+      float dgate[8], gate[8];
+      if (!kHold) weights(c);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[ch][j] = rf * fmaf(-f[ch][j], m, g[ch][j]);
+      for (int j = 0; j < 8; ++j) gate[j] = gt;
+      if (p.gate_mode == DSALT_GATE_FULL) load8<T, VEC>(Gt + at, p.d - c, gate);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float G = fmaf(-e, x[ch][j], u[ch][j]);
+        u[ch][j] = G;
+        const bool kept = keep[ch] >> j & 1u;
+        const float P = kept ? G * dr.scale : 0.f, fr = kept ? f[ch][j] * rf : 0.f;
+        const float n = fr * hp[j], Pg = P * gate[j], dn = Pg * hs[j];
+        a_post[ch][j] = fmaf(dn, fr, a_post[ch][j]);
+        a_scale[ch][j] = fmaf(Pg, n, a_scale[ch][j]);
+        dgate[j] = P * hs[j] * n;
+        f[ch][j] = p.post ? rf * fmaf(-f[ch][j], m, dn * hp[j]) : dn;
       }
-      store8<T, VEC>(reinterpret_cast<T*>(p.df) + t * p.d + c, p.d - c, g[ch]);
+      store8<T, VEC>(reinterpret_cast<T*>(p.dx) + at, p.d - c, u[ch]);
+      store8<T, VEC>(reinterpret_cast<T*>(p.df) + at, p.d - c, f[ch]);
+      if (p.gate_mode == DSALT_GATE_FULL) store8<T, VEC>(reinterpret_cast<T*>(p.dgate) + at, p.d - c, dgate);
     }
+    if (!kHold && k + 1 < rounds) fetch(t + stride);
   }
   // this group's sums: partial row `first` of [groups][3][d] (scale, post, norm)
   float* part = p.parts + first * 3 * p.d;
@@ -317,33 +375,38 @@ cudaError_t sm_count(int* out) {
   return cudaSuccess;
 }
 
-// CTAs of the backward: as many as run at once, no more than there are rows for
-int bwd_ctas(int64_t T, const Shape& s, int sms) {
+// CTAs that run at once: 16 warps an SM for the backward's registers, 32 for the
+// forward's; no more than there are rows for
+int64_t ctas_of(int64_t T, const Shape& s, int threads_per_sm, int sms) {
   const int per_cta = s.cta / s.group;
-  const int64_t want = (T + per_cta - 1) / per_cta;
-  const int64_t most = (int64_t)sms * (1024 / s.cta < 1 ? 1 : 1024 / s.cta);
-  return (int)(want < most ? want : most);
+  const int64_t want = (T + per_cta - 1) / per_cta, most = (int64_t)sms * (threads_per_sm / s.cta);
+  return want < most ? want : most;
 }
+constexpr int kBwdThreads = 512, kFwdThreads = 1024;
 
-template <typename T, int CH, bool VEC>
+template <typename T, int CH, bool VEC, int MAXT>
 cudaError_t launch_v(const DsaltResidualNormParams& p, const Shape& s, bool bwd, cudaStream_t st) {
   int sms = 0;
   cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
-  const int per_cta = s.cta / s.group;
   if (!bwd) {
-    const int64_t want = (p.T + per_cta - 1) / per_cta, most = (int64_t)sms * 2048 / s.cta;
-    residual_fwd_kernel<T, CH, VEC><<<(unsigned)(want < most ? want : most), s.cta, 0, st>>>(p, s.group);
+    residual_fwd_kernel<T, CH, VEC, MAXT><<<(unsigned)ctas_of(p.T, s, kFwdThreads, sms), s.cta, 0, st>>>(p, s.group);
     return cudaGetLastError();
   }
-  const int ctas = bwd_ctas(p.T, s, sms);
-  residual_bwd_kernel<T, CH, VEC><<<ctas, s.cta, 0, st>>>(p, s.group);
+  const int64_t ctas = ctas_of(p.T, s, kBwdThreads, sms);
+  residual_bwd_kernel<T, CH, VEC, MAXT><<<(unsigned)ctas, s.cta, 0, st>>>(p, s.group);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   if (p.dscale || p.dpost || p.dnorm) {
-    residual_colsum_kernel<T><<<dim3((p.d + 31) / 32, 3), 1024, 0, st>>>(p, (int64_t)ctas * per_cta);
+    residual_colsum_kernel<T><<<dim3((p.d + 31) / 32, 3), 1024, 0, st>>>(p, ctas * (s.cta / s.group));
     e = cudaGetLastError();
   }
   return e;
+}
+template <typename T, bool VEC>
+cudaError_t launch_s(const DsaltResidualNormParams& p, const Shape& s, bool bwd, cudaStream_t st) {
+  if (s.chunks == 4) return launch_v<T, 4, VEC, 512>(p, s, bwd, st);
+  if (s.chunks == 2) return launch_v<T, 2, VEC, 512>(p, s, bwd, st);
+  return s.cta > 256 ? launch_v<T, 1, VEC, 512>(p, s, bwd, st) : launch_v<T, 1, VEC, 256>(p, s, bwd, st);
 }
 
 template <typename T>
@@ -354,8 +417,7 @@ cudaError_t launch_t(const DsaltResidualNormParams& p, bool bwd, cudaStream_t st
                         (const void*)p.df, p.gate_mode == DSALT_GATE_FULL ? p.gate : nullptr,
                         p.gate_mode == DSALT_GATE_FULL ? (const void*)p.dgate : nullptr})
     vec = vec && ((uintptr_t)q & 15) == 0;
-  if (s.chunks == 1) return vec ? launch_v<T, 1, true>(p, s, bwd, st) : launch_v<T, 1, false>(p, s, bwd, st);
-  return vec ? launch_v<T, 2, true>(p, s, bwd, st) : launch_v<T, 2, false>(p, s, bwd, st);
+  return vec ? launch_s<T, true>(p, s, bwd, st) : launch_s<T, false>(p, s, bwd, st);
 }
 
 }  // namespace
@@ -365,7 +427,7 @@ cudaError_t residual_norm_parts(int64_t T, int d, int* out) {
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
   const Shape s = shape_of(d);
-  *out = bwd_ctas(T, s, sms) * (s.cta / s.group);
+  *out = (int)ctas_of(T, s, kBwdThreads, sms) * (s.cta / s.group);
   return cudaSuccess;
 }
 
