@@ -19,20 +19,20 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DsaltDropoutPar
   const T* x = reinterpret_cast<const T*>(p.x) + i;
   T* y = reinterpret_cast<T*>(p.y) + i;
   const int left = (int)min((int64_t)8, p.n - i);
-  const uint32_t keep = dr.keep_block((uint64_t)i >> 3);
-  float v[8];
-  if (VEC && left == 8) {
-    load8<T, true>(x, 8, v);
-  } else {
-    load8<T, false>(x, left, v);
-  }
+  uint32_t m[8];
+  dr.masks_block((uint64_t)i >> 3, m);
+  const f2 scale = pair(dr.scale, dr.scale);
+  auto drop = [&](auto raw) {
+    f2 v[4];
+    raw.load(x, left);
+    raw.get(v);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = (keep >> j & 1u) ? v[j] * dr.scale : 0.f;
-  if (VEC && left == 8) {
-    store8<T, true>(y, 8, v);
-  } else {
-    store8<T, false>(y, left, v);
-  }
+    for (int j = 0; j < 4; ++j) v[j] = mul2(and2(v[j], m[2 * j], m[2 * j + 1]), scale);
+    raw.set(v);
+    raw.store(y, left);
+  };
+  if (VEC && left == 8) drop(Raw<T, true>());
+  else drop(Raw<T, false>());
 }
 
 template <typename T>

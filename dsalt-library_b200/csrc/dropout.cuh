@@ -2,6 +2,8 @@
 // site, element index), so it is computed again wherever it is needed and never stored.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace dsalt {
@@ -34,62 +36,143 @@ struct Dropout {
     const uint64_t s = threshold_ > 0 ? (uint64_t)__ldg(seed) : 0;
     key = make_uint2((uint32_t)s, (uint32_t)(s >> 32));
   }
-  // bit j: element 8·block + j is kept
-  __device__ __forceinline__ uint32_t keep_block(uint64_t block) const {
+  // m[j] = all ones where element 8·block + j is kept, 0 where it is dropped
+  __device__ __forceinline__ void masks_block(uint64_t block, uint32_t* m) const {
     const uint4 w = philox(make_uint4((uint32_t)block, (uint32_t)(block >> 32), site, 0u), key);
     const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-    uint32_t m = 0;
+    if (threshold >= 65536) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m[j] = 0u;
+      return;
+    }
+    const uint32_t high = threshold << 16;  // draw >= threshold, compared in the upper halves
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      m |= (uint32_t)((v[j] & 0xffffu) >= threshold) << (2 * j);
-      m |= (uint32_t)((v[j] >> 16) >= threshold) << (2 * j + 1);
+      m[2 * j] = (v[j] << 16) >= high ? 0xffffffffu : 0u;
+      m[2 * j + 1] = v[j] >= high ? 0xffffffffu : 0u;
     }
-    return m;
   }
-  // bit j: element i + j is kept, 0 ≤ j < 8, any i
-  __device__ __forceinline__ uint32_t keep8(uint64_t i) const {
+  // the masks of elements i … i + 7, any i
+  __device__ __forceinline__ void masks8(uint64_t i, uint32_t* m) const {
     const uint32_t o = (uint32_t)i & 7u;
-    uint32_t m = keep_block(i >> 3);
-    if (o) m = (m | keep_block((i >> 3) + 1) << 8) >> o;
-    return m;
+    uint32_t a[16];
+    masks_block(i >> 3, a);
+    if (o) masks_block((i >> 3) + 1, a + 8);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      m[j] = a[j];
+#pragma unroll
+      for (int k = 1; k < 8; ++k)
+        if (o == k) m[j] = a[j + k];
+    }
   }
 };
 
-// ------------------------------------------------- eight consecutive elements
-// VEC: aligned 16-byte accesses and all eight inside; else element by element,
-// those at or past n (counted from the first) left out and read as 0.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int n, float* v) {
-  if constexpr (VEC && sizeof(T) == 2) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-    const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(e[j]);
-  } else if constexpr (VEC) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? to_f32<T>(p[j]) : 0.f;
-  }
+// Pairs of fp32 values for the packed fp32 instructions of sm_100.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pair(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
+__device__ __forceinline__ void unpair(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 and2(f2 v, uint32_t m0, uint32_t m1) { return v & ((f2)m1 << 32 | m0); }
+
+// ------------------------------------------------- eight consecutive elements
+// As they lie in memory, so that they can be on their way in few registers.  VEC:
+// aligned 16-byte accesses and all eight inside; else element by element, those at or
+// past n (counted from the first) read as 0 and not written.
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, int n, const float* v) {
-  if constexpr (VEC && sizeof(T) == 2) {
-    uint4 u;
-    T* e = reinterpret_cast<T*>(&u);
+struct Raw {
+  T e[8];
+  __device__ __forceinline__ void load(const T* p, int n) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(v[j]);
-    *reinterpret_cast<uint4*>(p) = u;
-  } else if constexpr (VEC) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
+    for (int j = 0; j < 8; ++j) e[j] = j < n ? p[j] : from_f32<T>(0.f);
+  }
+  __device__ __forceinline__ void zero() { load(nullptr, 0); }
+  __device__ __forceinline__ void get(f2* v) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = pair(to_f32<T>(e[2 * j]), to_f32<T>(e[2 * j + 1]));
+  }
+  __device__ __forceinline__ void set(const f2* v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float a, b;
+      unpair(v[j], a, b);
+      e[2 * j] = from_f32<T>(a);
+      e[2 * j + 1] = from_f32<T>(b);
+    }
+  }
+  __device__ __forceinline__ void store(T* p, int n) const {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = from_f32<T>(v[j]);
+      if (j < n) p[j] = e[j];
   }
-}
+};
+template <typename T>
+struct Raw<T, true> {
+  uint32_t w[2 * sizeof(T)];
+  __device__ __forceinline__ void load(const T* p, int) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < (int)(2 * sizeof(T)); ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void get(f2* v) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        v[j] = pair(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+      } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        v[j] = pair(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+      } else {
+        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        v[j] = pair(h.x, h.y);
+      }
+    }
+  }
+  __device__ __forceinline__ void set(const f2* v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float a, b;
+      unpair(v[j], a, b);
+      if constexpr (sizeof(T) == 4) {
+        w[2 * j] = __float_as_uint(a);
+        w[2 * j + 1] = __float_as_uint(b);
+      } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        w[j] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(a, b);
+        w[j] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* p, int) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+      reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  }
+};
 
 }  // namespace dsalt

@@ -20,6 +20,8 @@
 // (for df and a token's dgate; κ there without the token's gate) after it.  G = u − e·x' with u = dx_new + r·dh⊙norm and
 // e = r³·mean(dh⊙norm⊙x') is linear in that first sum, so Σ κ⊙G = Σ κ⊙u − e·Σ κ⊙x':
 // one round of three sums a row instead of two dependent rounds.
+// dscale and dpost share one sum over the rows, A = Σ_t D(G)⊙gate⊙f·rf: dscale = post⊙A,
+// dpost = scale⊙A.
 #include "dropout.cuh"
 
 namespace dsalt {
@@ -41,39 +43,6 @@ inline Shape shape_of(int d) {
   const int t = ((units + chunks - 1) / chunks + 31) / 32 * 32;
   return {t, t, chunks};
 }
-
-// Eight consecutive elements of a row as they lie in memory, so that the next row's
-// can be on their way in few registers.
-template <typename T, bool VEC>
-struct Raw {
-  T e[8];
-  __device__ __forceinline__ void load(const T* p, int n) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = j < n ? p[j] : from_f32<T>(0.f);
-  }
-  __device__ __forceinline__ void zero() { load(nullptr, 0); }
-  __device__ __forceinline__ void get(float* v) const {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(e[j]);
-  }
-};
-template <typename T>
-struct Raw<T, true> {
-  uint4 u[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p, int) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = make_uint4(0, 0, 0, 0);
-  }
-  __device__ __forceinline__ void get(float* v) const {
-    const T* e = reinterpret_cast<const T*>(u);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(e[j]);
-  }
-};
 
 // Sums over the row group, NV values at once; every thread gets the totals.  `red`: one
 // of two halves that calls use in turn, so that a call needs one barrier: a half is
@@ -98,6 +67,7 @@ __device__ __forceinline__ void group_sum(float (&v)[NV], int group, float* red)
     for (int k = 0; k < NV; ++k) v[k] += red[w * NV + k];
 }
 
+// weights of eight columns from c (1 without a vector, and past d)
 template <typename T>
 __device__ __forceinline__ void load_weights(const void* w, bool f32, int c, int d, float* v) {
 #pragma unroll
@@ -106,11 +76,42 @@ __device__ __forceinline__ void load_weights(const void* w, bool f32, int c, int
                                  : to_f32<T>(reinterpret_cast<const T*>(w)[c + j]))
                           : 1.f;
 }
+// post·scale·(1 / share kept) and norm of this thread's columns
+template <typename T>
+__device__ __forceinline__ void column_factors(const DsaltResidualNormParams& p, const Dropout& dr, int c, f2* branch,
+                                               f2* norm) {
+  float a[8], b[8];
+  load_weights<T>(p.post, p.w_f32, c, p.d, a);
+  load_weights<T>(p.scale, p.w_f32, c, p.d, b);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) branch[j] = pair(a[2 * j] * b[2 * j] * dr.scale, a[2 * j + 1] * b[2 * j + 1] * dr.scale);
+  load_weights<T>(p.norm, p.w_f32, c, p.d, a);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) norm[j] = pair(a[2 * j], a[2 * j + 1]);
+}
+template <bool VEC>
+__device__ __forceinline__ void row_masks(const Dropout& dr, int64_t at, uint32_t* m) {
+  if (dr.threshold == 0) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m[j] = 0xffffffffu;
+  } else if (VEC) {
+    dr.masks_block((uint64_t)at >> 3, m);
+  } else {
+    dr.masks8((uint64_t)at, m);
+  }
+}
+__device__ __forceinline__ f2 dup(float v) { return pair(v, v); }
+__device__ __forceinline__ float sum8(f2 s) {
+  float a, b;
+  unpair(s, a, b);
+  return a + b;
+}
 
 constexpr int kMaxWarps = 16;
 
 template <typename T, int CH, bool VEC, int MAXT>
-__global__ void __launch_bounds__(MAXT) residual_fwd_kernel(const DsaltResidualNormParams p, int group) {
+__global__ void __launch_bounds__(MAXT, 1024 / MAXT) residual_fwd_kernel(const DsaltResidualNormParams p, int group) {
+  constexpr bool kHold = CH == 1;  // weights in registers, the next row's loads early
   __shared__ float red[2][kMaxWarps];
   const int gid = threadIdx.x / group, lane = threadIdx.x - gid * group, per_cta = blockDim.x / group;
   const int64_t stride = (int64_t)gridDim.x * per_cta;
@@ -122,18 +123,8 @@ __global__ void __launch_bounds__(MAXT) residual_fwd_kernel(const DsaltResidualN
   const T* Fv = reinterpret_cast<const T*>(p.f);
   const T* Gt = reinterpret_cast<const T*>(p.gate);
   const float inv_d = 1.f / (float)p.d;
-  // post·scale and norm of this thread's columns
-  float ws[CH][8], wn[CH][8];
-#pragma unroll
-  for (int ch = 0; ch < CH; ++ch) {
-    const int c = (lane + ch * group) * 8;
-    float w[8];
-    load_weights<T>(p.post, p.w_f32, c, p.d, w);
-    load_weights<T>(p.scale, p.w_f32, c, p.d, ws[ch]);
-    load_weights<T>(p.norm, p.w_f32, c, p.d, wn[ch]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ws[ch][j] *= w[j];
-  }
+  f2 wb[4], wn[4];
+  if (kHold) column_factors<T>(p, dr, lane * 8, wb, wn);
   Raw<T, VEC> nx[CH], nf[CH];
   auto fetch = [&](int64_t t) {
 #pragma unroll
@@ -152,44 +143,54 @@ __global__ void __launch_bounds__(MAXT) residual_fwd_kernel(const DsaltResidualN
   fetch(t);
   for (int64_t k = 0; k < rounds; ++k, t += stride) {
     const bool on = t < p.T;
-    float f[CH][8], x[CH][8], s[1] = {0.f};
+    f2 f[CH][4], x[CH][4], s2 = dup(0.f);
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       nf[ch].get(f[ch]);
       nx[ch].get(x[ch]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[0] = fmaf(f[ch][j], f[ch][j], s[0]);
+      for (int j = 0; j < 4; ++j) s2 = fma2(f[ch][j], f[ch][j], s2);
     }
-    if (k + 1 < rounds) fetch(t + stride);
+    if (kHold && k + 1 < rounds) fetch(t + stride);
     float rf = 1.f;
     if (p.post) {
+      float s[1] = {sum8(s2)};
       group_sum(s, group, red[0]);
       rf = rsqrtf(fmaf(s[0], inv_d, p.eps));
       if (on && lane == 0 && p.rf) p.rf[t] = rf;
     }
     if (p.gate_mode == DSALT_GATE_TOKEN && on) rf *= to_f32<T>(Gt[t]);
-    s[0] = 0.f;
+    const f2 rf2 = dup(rf);
+    s2 = dup(0.f);
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (lane + ch * group) * 8;
       if (!(on && c < p.d)) continue;
       const int64_t at = t * p.d + c;
+      if (!kHold) column_factors<T>(p, dr, c, wb, wn);
+      uint32_t m[8];
+      row_masks<VEC>(dr, at, m);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[ch][j] = mul2(and2(f[ch][j], m[2 * j], m[2 * j + 1]), wb[j]);
       if (p.gate_mode == DSALT_GATE_FULL) {
-        float w[8];
-        load8<T, VEC>(Gt + at, p.d - c, w);
+        Raw<T, VEC> raw;
+        f2 g[4];
+        raw.load(Gt + at, p.d - c);
+        raw.get(g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[ch][j] *= w[j];
+        for (int j = 0; j < 4; ++j) f[ch][j] = mul2(f[ch][j], and2(g[j], m[2 * j], m[2 * j + 1]));
       }
-      const uint32_t keep = p.threshold > 0 ? (VEC ? dr.keep_block((uint64_t)at >> 3) : dr.keep8((uint64_t)at)) : 0xffu;
+      Raw<T, VEC> out;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float a = f[ch][j] * (ws[ch][j] * rf);
-        x[ch][j] = round_to<T>((keep >> j & 1u) ? fmaf(a, dr.scale, x[ch][j]) : x[ch][j]);
-        s[0] = fmaf(x[ch][j], x[ch][j], s[0]);
-      }
-      store8<T, VEC>(reinterpret_cast<T*>(p.x_new) + at, p.d - c, x[ch]);
+      for (int j = 0; j < 4; ++j) x[ch][j] = fma2(f[ch][j], rf2, x[ch][j]);
+      out.set(x[ch]);
+      out.store(reinterpret_cast<T*>(p.x_new) + at, p.d - c);
+      out.get(x[ch]);  // the rounded x'
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s2 = fma2(x[ch][j], x[ch][j], s2);
     }
     if (p.norm) {
+      float s[1] = {sum8(s2)};
       group_sum(s, group, red[1]);
       const float r = rsqrtf(fmaf(s[0], inv_d, p.eps));
       if (on && lane == 0 && p.r) p.r[t] = r;
@@ -197,20 +198,22 @@ __global__ void __launch_bounds__(MAXT) residual_fwd_kernel(const DsaltResidualN
       for (int ch = 0; ch < CH; ++ch) {
         const int c = (lane + ch * group) * 8;
         if (!(on && c < p.d)) continue;
+        if (!kHold) column_factors<T>(p, dr, c, wb, wn);
+        Raw<T, VEC> out;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[ch][j] = x[ch][j] * r * wn[ch][j];
-        store8<T, VEC>(reinterpret_cast<T*>(p.h) + t * p.d + c, p.d - c, x[ch]);
+        for (int j = 0; j < 4; ++j) x[ch][j] = mul2(mul2(x[ch][j], dup(r)), wn[j]);
+        out.set(x[ch]);
+        out.store(reinterpret_cast<T*>(p.h) + t * p.d + c, p.d - c);
       }
     }
-    // with one sum a row the halves still alternate row by row
+    if (!kHold && k + 1 < rounds) fetch(t + stride);
+    // with one sum a row the next row's would write what this row's may still read
     if (!(p.post && p.norm) && group > 32) __syncthreads();
   }
 }
 
 template <typename T, int CH, bool VEC, int MAXT>
 __global__ void __launch_bounds__(MAXT, 512 / MAXT) residual_bwd_kernel(const DsaltResidualNormParams p, int group) {
-  // one chunk a thread: its weights stay in registers and the next row's loads go out
-  // early; with more chunks the registers are left to the column sums
   constexpr bool kHold = CH == 1;
   __shared__ float red[2][3 * kMaxWarps];
   const int gid = threadIdx.x / group, lane = threadIdx.x - gid * group, per_cta = blockDim.x / group;
@@ -219,19 +222,15 @@ __global__ void __launch_bounds__(MAXT, 512 / MAXT) residual_bwd_kernel(const Ds
   Dropout dr;
   dr.init(p.seed, p.site, p.threshold);
   const T* Gt = reinterpret_cast<const T*>(p.gate);
-  const bool with_h = p.norm && p.dh, sums = with_h || p.post || p.gate_mode == DSALT_GATE_TOKEN;
+  const bool with_h = p.norm && p.dh, full = p.gate_mode == DSALT_GATE_FULL;
+  const bool sums = with_h || p.post || p.gate_mode == DSALT_GATE_TOKEN;
   const float inv_d = 1.f / (float)p.d;
-  float hp[8], hs[8], hn[8], a_scale[CH][8], a_post[CH][8], a_norm[CH][8];
-  auto weights = [&](int c) {
-    load_weights<T>(p.post, p.w_f32, c, p.d, hp);
-    load_weights<T>(p.scale, p.w_f32, c, p.d, hs);
-    load_weights<T>(p.norm, p.w_f32, c, p.d, hn);
-  };
-  if (kHold) weights(lane * 8);
+  f2 wb[4], wn[4], a_branch[CH][4], a_norm[CH][4];
+  if (kHold) column_factors<T>(p, dr, lane * 8, wb, wn);
 #pragma unroll
   for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a_scale[ch][j] = a_post[ch][j] = a_norm[ch][j] = 0.f;
+    for (int j = 0; j < 4; ++j) a_branch[ch][j] = a_norm[ch][j] = dup(0.f);
   Raw<T, VEC> nx[CH], nf[CH], nd[CH], nh[CH];  // x', f, dx_new, dh
   float nr = 0.f, nrf = 1.f, ngt = 1.f;
   auto fetch = [&](int64_t t) {
@@ -259,106 +258,140 @@ __global__ void __launch_bounds__(MAXT, 512 / MAXT) residual_bwd_kernel(const Ds
   for (int64_t k = 0; k < rounds; ++k, t += stride) {
     const bool on = t < p.T;
     const float r = nr, rf = nrf, gt = ngt;
-    float u[CH][8], x[CH][8], f[CH][8];
-    uint32_t keep[CH];
-    float s[3] = {0.f, 0.f, 0.f};
+    const f2 r2 = dup(r);
+    f2 u[CH][4], x[CH][4], f[CH][4];
+    uint32_t m[CH][8];
+    f2 s0 = dup(0.f), s1 = dup(0.f), s2 = dup(0.f);
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (lane + ch * group) * 8;
       const int64_t at = t * p.d + c;
-      float dh[8], gate[8];
+      f2 dh[4], g[4] = {dup(1.f), dup(1.f), dup(1.f), dup(1.f)};
       nx[ch].get(x[ch]);
       nf[ch].get(f[ch]);
       nd[ch].get(u[ch]);
       nh[ch].get(dh);
-      if (!kHold) weights(c);
-      keep[ch] = p.threshold > 0 ? (VEC ? dr.keep_block((uint64_t)at >> 3) : dr.keep8((uint64_t)at)) : 0xffu;
+      if (!kHold) column_factors<T>(p, dr, c, wb, wn);
+      row_masks<VEC>(dr, at, m[ch]);
+      if (full && on && c < p.d) {
+        Raw<T, VEC> raw;
+        raw.load(Gt + at, p.d - c);
+        raw.get(g);
+      }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) gate[j] = 1.f;
-      if (p.gate_mode == DSALT_GATE_FULL && on && c < p.d) load8<T, VEC>(Gt + at, p.d - c, gate);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float q = dh[j] * hn[j];
-        a_norm[ch][j] = fmaf(dh[j], x[ch][j] * r, a_norm[ch][j]);
-        s[0] = fmaf(q, x[ch][j], s[0]);
-        u[ch][j] = fmaf(r, q, u[ch][j]);
-        // a dropped element passes nothing back, whatever f holds there
-        const float kf = (keep[ch] >> j & 1u) ? f[ch][j] * hp[j] * (dr.scale * hs[j]) * gate[j] : 0.f;
-        s[1] = fmaf(kf, u[ch][j], s[1]);
-        s[2] = fmaf(kf, x[ch][j], s[2]);
+      for (int j = 0; j < 4; ++j) {
+        const f2 hx = mul2(dh[j], x[ch][j]);
+        a_norm[ch][j] = fma2(hx, r2, a_norm[ch][j]);
+        s0 = fma2(hx, wn[j], s0);
+        u[ch][j] = fma2(mul2(dh[j], wn[j]), r2, u[ch][j]);
+        // κ: a dropped element passes nothing back, whatever f holds there
+        f2 kf = and2(f[ch][j], m[ch][2 * j], m[ch][2 * j + 1]);
+        if (!p.post) f[ch][j] = kf;
+        kf = mul2(kf, wb[j]);
+        if (full) kf = mul2(kf, g[j]);
+        s1 = fma2(kf, u[ch][j], s1);
+        s2 = fma2(kf, x[ch][j], s2);
       }
     }
     if (kHold && k + 1 < rounds) fetch(t + stride);
+    float s[3] = {sum8(s0), sum8(s1), sum8(s2)};
     if (sums) group_sum(s, group, red[k & 1]);
     const float e = r * r * r * (s[0] * inv_d);
     const float S = fmaf(-e, s[2], s[1]);  // Σ κ⊙G, without a token's gate
     if (p.gate_mode == DSALT_GATE_TOKEN && on && lane == 0) reinterpret_cast<T*>(p.dgate)[t] = from_f32<T>(rf * S);
-    const float m = rf * rf * gt * (S * inv_d);
+    const f2 ne = dup(-e), al = dup(rf * gt), nm = dup(-rf * rf * rf * gt * (S * inv_d));
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (lane + ch * group) * 8;
       if (!(on && c < p.d)) continue;
       const int64_t at = t * p.d + c;
-      float dgate[8], gate[8];
-      if (!kHold) weights(c);
+      if (!kHold) column_factors<T>(p, dr, c, wb, wn);
+      Raw<T, VEC> out;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) gate[j] = gt;
-      if (p.gate_mode == DSALT_GATE_FULL) load8<T, VEC>(Gt + at, p.d - c, gate);
+      for (int j = 0; j < 4; ++j) u[ch][j] = fma2(ne, x[ch][j], u[ch][j]);  // G
+      out.set(u[ch]);
+      out.store(reinterpret_cast<T*>(p.dx) + at, p.d - c);
+      f2 df[4];
+      if (full) {
+        f2 g[4], dg[4];
+        out.load(Gt + at, p.d - c);
+        out.get(g);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float G = fmaf(-e, x[ch][j], u[ch][j]);
-        u[ch][j] = G;
-        const bool kept = keep[ch] >> j & 1u;
-        const float P = kept ? G * dr.scale : 0.f, fr = kept ? f[ch][j] * rf : 0.f;
-        const float n = fr * hp[j], Pg = P * gate[j], dn = Pg * hs[j];
-        a_post[ch][j] = fmaf(dn, fr, a_post[ch][j]);
-        a_scale[ch][j] = fmaf(Pg, n, a_scale[ch][j]);
-        dgate[j] = P * hs[j] * n;
-        f[ch][j] = p.post ? rf * fmaf(-f[ch][j], m, dn * hp[j]) : dn;
+        for (int j = 0; j < 4; ++j) {
+          const f2 G = and2(u[ch][j], m[ch][2 * j], m[ch][2 * j + 1]);
+          const f2 Gw = mul2(G, wb[j]);
+          dg[j] = mul2(mul2(Gw, f[ch][j]), al);
+          df[j] = mul2(mul2(Gw, g[j]), al);
+          a_branch[ch][j] = fma2(mul2(mul2(G, g[j]), f[ch][j]), al, a_branch[ch][j]);
+        }
+        out.set(dg);
+        out.store(reinterpret_cast<T*>(p.dgate) + at, p.d - c);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f2 G = and2(u[ch][j], m[ch][2 * j], m[ch][2 * j + 1]);
+          df[j] = mul2(mul2(G, wb[j]), al);
+          a_branch[ch][j] = fma2(mul2(G, f[ch][j]), al, a_branch[ch][j]);
+        }
       }
-      store8<T, VEC>(reinterpret_cast<T*>(p.dx) + at, p.d - c, u[ch]);
-      store8<T, VEC>(reinterpret_cast<T*>(p.df) + at, p.d - c, f[ch]);
-      if (p.gate_mode == DSALT_GATE_FULL) store8<T, VEC>(reinterpret_cast<T*>(p.dgate) + at, p.d - c, dgate);
+      if (p.post) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) df[j] = fma2(f[ch][j], nm, df[j]);
+      }
+      out.set(df);
+      out.store(reinterpret_cast<T*>(p.df) + at, p.d - c);
     }
     if (!kHold && k + 1 < rounds) fetch(t + stride);
   }
-  // this group's sums: partial row `first` of [groups][3][d] (scale, post, norm)
-  float* part = p.parts + first * 3 * p.d;
+  // this group's sums: partial row `first` of [groups][2][d] (Σ G⊙gate⊙f·rf where kept, Σ dh⊙x'·r)
+  float* part = p.parts + first * 2 * p.d;
 #pragma unroll
   for (int ch = 0; ch < CH; ++ch) {
     const int c = (lane + ch * group) * 8;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (c + j >= p.d) continue;
-      part[c + j] = a_scale[ch][j];
-      part[p.d + c + j] = a_post[ch][j];
-      part[2 * p.d + c + j] = a_norm[ch][j];
+    for (int j = 0; j < 4; ++j) {
+      float a, b, n0, n1;
+      unpair(a_branch[ch][j], a, b);
+      unpair(a_norm[ch][j], n0, n1);
+      if (c + 2 * j < p.d) part[c + 2 * j] = a, part[p.d + c + 2 * j] = n0;
+      if (c + 2 * j + 1 < p.d) part[c + 2 * j + 1] = b, part[p.d + c + 2 * j + 1] = n1;
     }
   }
 }
 
 // Column sums of the partial rows in a fixed order: a CTA owns 32 columns of one of
-// the three vectors; warp w adds rows w, w + 32, …, then the warps' sums in order.
+// the two sums; warp w adds rows w, w + 32, …, then the warps' sums in order.  The first
+// sum, times 1 / share kept, gives dscale with post's weights and dpost with scale's.
 template <typename T>
 __global__ void __launch_bounds__(1024) residual_colsum_kernel(const DsaltResidualNormParams p, int64_t nparts) {
-  void* out = blockIdx.y == 0 ? p.dscale : blockIdx.y == 1 ? p.dpost : p.dnorm;
-  if (!out) return;
   __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float acc = 0.f;
   if (c < p.d)
 #pragma unroll 8
-    for (int64_t i = grp; i < nparts; i += 32) acc += __ldg(p.parts + (i * 3 + blockIdx.y) * p.d + c);
+    for (int64_t i = grp; i < nparts; i += 32) acc += __ldg(p.parts + (i * 2 + blockIdx.y) * p.d + c);
   s[grp][lane] = acc;
   __syncthreads();
-  if (grp == 0 && c < p.d) {
-    float v = 0.f;
+  if (grp != 0 || c >= p.d) return;
+  float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < 32; ++w) v += s[w][lane];
-    if (p.w_f32) reinterpret_cast<float*>(out)[c] = v;
-    else reinterpret_cast<T*>(out)[c] = from_f32<T>(v);
+  for (int w = 0; w < 32; ++w) v += s[w][lane];
+  auto weight = [&](const void* w) {
+    return !w ? 1.f : p.w_f32 ? __ldg(reinterpret_cast<const float*>(w) + c) : to_f32<T>(reinterpret_cast<const T*>(w)[c]);
+  };
+  auto put = [&](void* out, float x) {
+    if (!out) return;
+    if (p.w_f32) reinterpret_cast<float*>(out)[c] = x;
+    else reinterpret_cast<T*>(out)[c] = from_f32<T>(x);
+  };
+  if (blockIdx.y == 1) {
+    put(p.dnorm, v);
+    return;
   }
+  v *= p.threshold >= 65536 ? 0.f : 65536.f / (float)(65536 - p.threshold);
+  put(p.dscale, v * weight(p.post));
+  put(p.dpost, v * weight(p.scale));
 }
 
 cudaError_t sm_count(int* out) {
@@ -397,7 +430,7 @@ cudaError_t launch_v(const DsaltResidualNormParams& p, const Shape& s, bool bwd,
   residual_bwd_kernel<T, CH, VEC, MAXT><<<(unsigned)ctas, s.cta, 0, st>>>(p, s.group);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   if (p.dscale || p.dpost || p.dnorm) {
-    residual_colsum_kernel<T><<<dim3((p.d + 31) / 32, 3), 1024, 0, st>>>(p, ctas * (s.cta / s.group));
+    residual_colsum_kernel<T><<<dim3((p.d + 31) / 32, p.dnorm ? 2 : 1), 1024, 0, st>>>(p, ctas * (s.cta / s.group));
     e = cudaGetLastError();
   }
   return e;

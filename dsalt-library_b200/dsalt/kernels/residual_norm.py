@@ -75,7 +75,7 @@ class ResidualNormFunction(torch.autograd.Function):
             n = _ext.load().dsalt_residual_norm_parts(p.T, p.d)
         if n < 0:
             raise RuntimeError(f"dsalt_residual_norm_parts failed: {_ext.status_string(-n)}")
-        parts = torch.empty(max(n, 1), 3, p.d, dtype=torch.float32, device=f.device)
+        parts = torch.empty(max(n, 1), 2, p.d, dtype=torch.float32, device=f.device)
         p.rf, p.r, p.dx_new, p.dh = _ext.ptr(rf), _ext.ptr(r), _ext.ptr(dx_new), _ext.ptr(dh)
         p.dx, p.df, p.dgate, p.parts = dx.data_ptr(), df.data_ptr(), _ext.ptr(dgate), parts.data_ptr()
         p.dpost, p.dscale, p.dnorm = _ext.ptr(dpost), _ext.ptr(dscale), _ext.ptr(dnorm)

@@ -561,7 +561,7 @@ DSALT_API int dsalt_dropout(const DsaltDropoutParams* p, void* stream);
  *   dgate = D(G)⊙scale⊙n (summed over the columns for a gate per token),
  *   dscale = Σ_t D(G)⊙gate⊙n,  dpost = Σ_t dn⊙f·rf,  dnorm = Σ_t dh⊙x'·r,
  * all in fp32 with one rounding each; the Σ_t in a fixed order through `parts`
- * (dsalt_residual_norm_parts(T, d) rows of 3·d fp32).  f16 / bf16 / f32, any d up to
+ * (dsalt_residual_norm_parts(T, d) rows of 2·d fp32).  f16 / bf16 / f32, any d up to
  * DSALT_RESIDUAL_MAX_D; dense rows.                                          */
 #define DSALT_RESIDUAL_MAX_D 16384
 enum { DSALT_GATE_NONE = 0, DSALT_GATE_TOKEN = 1, DSALT_GATE_FULL = 2 };

@@ -278,7 +278,7 @@ def test_results_end_where_the_tensors_end():
     mark = 7.0
     x_new, h, dx, df = (torch.full((T + 3, d), mark, device="cuda", dtype=torch.bfloat16) for _ in range(4))
     r = torch.full((T + 3,), mark, device="cuda")
-    parts = torch.empty(_ext.load().dsalt_residual_norm_parts(T, d), 3, d, device="cuda")
+    parts = torch.empty(_ext.load().dsalt_residual_norm_parts(T, d), 2, d, device="cuda")
     P = _ext.ptr
     p = _ext.ResidualNormParams(x=P(t["x"]), f=P(t["f"]), norm=P(t["norm"]), x_new=P(x_new), h=P(h), r=P(r), dx=P(dx),
                                 df=P(df), dx_new=P(dx_new), dh=P(dh), parts=P(parts), T=T, d=d, eps=1e-6,
