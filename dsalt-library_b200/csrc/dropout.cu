@@ -9,36 +9,53 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// one thread per eight elements, a block of the generator
+// A thread takes kBlocks blocks of eight elements (a counter's draws each), a CTA's
+// width apart, with their loads out before the first draw: one block a thread left the
+// memory waiting for loads (18 us for 16384 × 1024 bf16, DROP_US with kBlocks).
+constexpr int kBlocks = 4;
+
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const DsaltDropoutParams p) {
-  const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 8;
-  if (i >= p.n) return;
+  const int64_t first = ((int64_t)blockIdx.x * kBlocks * kThreads + threadIdx.x) * 8;
   Dropout dr;
   dr.init(p.seed, p.site, p.threshold);
-  const T* x = reinterpret_cast<const T*>(p.x) + i;
-  T* y = reinterpret_cast<T*>(p.y) + i;
-  const int left = (int)min((int64_t)8, p.n - i);
-  uint32_t m[8];
-  dr.masks_block((uint64_t)i >> 3, m);
+  const T* x = reinterpret_cast<const T*>(p.x);
+  T* y = reinterpret_cast<T*>(p.y);
   const f2 scale = pair(dr.scale, dr.scale);
-  auto drop = [&](auto raw) {
+  auto drop = [&](auto& raw, int64_t i) {
+    uint32_t m[8];
     f2 v[4];
-    raw.load(x, left);
+    dr.masks_block((uint64_t)i >> 3, m);
     raw.get(v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = mul2(and2(v[j], m[2 * j], m[2 * j + 1]), scale);
     raw.set(v);
-    raw.store(y, left);
   };
-  if (VEC && left == 8) drop(Raw<T, true>());
-  else drop(Raw<T, false>());
+  if (VEC && first + ((kBlocks - 1) * kThreads + 1) * 8 <= p.n) {
+    Raw<T, true> raw[kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) raw[b].load(x + first + b * kThreads * 8, 8);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+      drop(raw[b], first + b * kThreads * 8);
+      raw[b].store(y + first + b * kThreads * 8, 8);
+    }
+    return;
+  }
+  for (int64_t i = first; i < p.n && i <= first + (kBlocks - 1) * kThreads * 8; i += kThreads * 8) {
+    const int left = (int)min((int64_t)8, p.n - i);
+    Raw<T, false> raw;
+    raw.load(x + i, left);
+    drop(raw, i);
+    raw.store(y + i, left);
+  }
 }
 
 template <typename T>
 cudaError_t launch_t(const DsaltDropoutParams& p, cudaStream_t st) {
   const bool vec = ((uintptr_t)p.x & 15) == 0 && ((uintptr_t)p.y & 15) == 0;
-  const unsigned grid = (unsigned)((p.n + 8 * kThreads - 1) / (8 * kThreads));
+  const int64_t per_cta = 8 * kBlocks * kThreads;
+  const unsigned grid = (unsigned)((p.n + per_cta - 1) / per_cta);
   if (vec) dropout_kernel<T, true><<<grid, kThreads, 0, st>>>(p);
   else dropout_kernel<T, false><<<grid, kThreads, 0, st>>>(p);
   return cudaGetLastError();

@@ -44,27 +44,42 @@ inline Shape shape_of(int d) {
   return {t, t, chunks};
 }
 
+constexpr int kMaxWarps = 16;
+
 // Sums over the row group, NV values at once; every thread gets the totals.  `red`: one
 // of two halves that calls use in turn, so that a call needs one barrier: a half is
-// written again only after the barrier of the call between.
+// written again only after the barrier of the call between.  A half has kMaxWarps
+// entries of NV (3: 4) values; those past the group's warps stay 0.
 template <int NV>
-__device__ __forceinline__ void group_sum(float (&v)[NV], int group, float* red) {
+__device__ __forceinline__ void group_sum(float (&v)[NV], int group, float4* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     if (o < group)
 #pragma unroll
       for (int k = 0; k < NV; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
   if (group <= 32) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = group >> 5;
-  if (lane == 0)
-#pragma unroll
-    for (int k = 0; k < NV; ++k) red[warp * NV + k] = v[k];
+  const int warp = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0) {
+    if constexpr (NV == 1) reinterpret_cast<float*>(red)[warp] = v[0];
+    else red[warp] = make_float4(v[0], v[1], v[2], 0.f);
+  }
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < NV; ++k) v[k] = 0.f;
-  for (int w = 0; w < nw; ++w)
+  for (int w = 0; w * 32 < group; w += 4) {
+    if constexpr (NV == 1) {
+      const float4 a = red[w / 4];
+      v[0] += (a.x + a.y) + (a.z + a.w);
+    } else {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) v[k] += red[w * NV + k];
+      for (int i = 0; i < 4; ++i) {
+        const float4 a = red[w + i];
+        v[0] += a.x;
+        v[1] += a.y;
+        v[2] += a.z;
+      }
+    }
+  }
 }
 
 // weights of eight columns from c (1 without a vector, and past d)
@@ -89,12 +104,12 @@ __device__ __forceinline__ void column_factors(const DsaltResidualNormParams& p,
 #pragma unroll
   for (int j = 0; j < 4; ++j) norm[j] = pair(a[2 * j], a[2 * j + 1]);
 }
-template <bool VEC>
+template <bool VEC, bool DROP>
 __device__ __forceinline__ void row_masks(const Dropout& dr, int64_t at, uint32_t* m) {
-  if (dr.threshold == 0) {
+  if constexpr (!DROP) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) m[j] = 0xffffffffu;
-  } else if (VEC) {
+  } else if constexpr (VEC) {
     dr.masks_block((uint64_t)at >> 3, m);
   } else {
     dr.masks8((uint64_t)at, m);
@@ -107,16 +122,17 @@ __device__ __forceinline__ float sum8(f2 s) {
   return a + b;
 }
 
-constexpr int kMaxWarps = 16;
-
-template <typename T, int CH, bool VEC, int MAXT>
+// DROP, POST: the parts that cost most where they are not wanted.
+template <typename T, int CH, bool VEC, int MAXT, bool DROP, bool POST>
 __global__ void __launch_bounds__(MAXT, 1024 / MAXT) residual_fwd_kernel(const DsaltResidualNormParams p, int group) {
   constexpr bool kHold = CH == 1;  // weights in registers, the next row's loads early
-  __shared__ float red[2][kMaxWarps];
+  __shared__ float4 red[2][kMaxWarps / 4];
+  if (threadIdx.x < 2 * kMaxWarps / 4) red[0][threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  __syncthreads();
   const int gid = threadIdx.x / group, lane = threadIdx.x - gid * group, per_cta = blockDim.x / group;
   const int64_t stride = (int64_t)gridDim.x * per_cta;
   // every group of a CTA makes the same number of rounds (the sums synchronise)
-  const int64_t rounds = (p.T - (int64_t)blockIdx.x * per_cta + stride - 1) / stride;
+  const int rounds = (int)((p.T - (int64_t)blockIdx.x * per_cta + stride - 1) / stride);
   Dropout dr;
   dr.init(p.seed, p.site, p.threshold);
   const T* X = reinterpret_cast<const T*>(p.x);
@@ -126,13 +142,13 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) residual_fwd_kernel(const D
   f2 wb[4], wn[4];
   if (kHold) column_factors<T>(p, dr, lane * 8, wb, wn);
   Raw<T, VEC> nx[CH], nf[CH];
-  auto fetch = [&](int64_t t) {
+  auto fetch = [&](int64_t t, int64_t row) {
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (lane + ch * group) * 8;
       if (t < p.T && c < p.d) {
-        nx[ch].load(X + t * p.d + c, p.d - c);
-        nf[ch].load(Fv + t * p.d + c, p.d - c);
+        nx[ch].load(X + row + c, p.d - c);
+        nf[ch].load(Fv + row + c, p.d - c);
       } else {
         nx[ch].zero();
         nf[ch].zero();
@@ -140,8 +156,9 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) residual_fwd_kernel(const D
     }
   };
   int64_t t = (int64_t)blockIdx.x * per_cta + gid;
-  fetch(t);
-  for (int64_t k = 0; k < rounds; ++k, t += stride) {
+  int64_t row = t * p.d;  // index of the row's first element
+  fetch(t, row);
+  for (int k = 0; k < rounds; ++k, t += stride, row += stride * p.d) {
     const bool on = t < p.T;
     f2 f[CH][4], x[CH][4], s2 = dup(0.f);
 #pragma unroll
@@ -151,9 +168,9 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) residual_fwd_kernel(const D
 #pragma unroll
       for (int j = 0; j < 4; ++j) s2 = fma2(f[ch][j], f[ch][j], s2);
     }
-    if (kHold && k + 1 < rounds) fetch(t + stride);
+    if (kHold && k + 1 < rounds) fetch(t + stride, row + stride * p.d);
     float rf = 1.f;
-    if (p.post) {
+    if (POST) {
       float s[1] = {sum8(s2)};
       group_sum(s, group, red[0]);
       rf = rsqrtf(fmaf(s[0], inv_d, p.eps));
@@ -166,10 +183,10 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) residual_fwd_kernel(const D
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (lane + ch * group) * 8;
       if (!(on && c < p.d)) continue;
-      const int64_t at = t * p.d + c;
+      const int64_t at = row + c;
       if (!kHold) column_factors<T>(p, dr, c, wb, wn);
       uint32_t m[8];
-      row_masks<VEC>(dr, at, m);
+      row_masks<VEC, DROP>(dr, at, m);
 #pragma unroll
       for (int j = 0; j < 4; ++j) f[ch][j] = mul2(and2(f[ch][j], m[2 * j], m[2 * j + 1]), wb[j]);
       if (p.gate_mode == DSALT_GATE_FULL) {
@@ -203,27 +220,29 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) residual_fwd_kernel(const D
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[ch][j] = mul2(mul2(x[ch][j], dup(r)), wn[j]);
         out.set(x[ch]);
-        out.store(reinterpret_cast<T*>(p.h) + t * p.d + c, p.d - c);
+        out.store(reinterpret_cast<T*>(p.h) + row + c, p.d - c);
       }
     }
-    if (!kHold && k + 1 < rounds) fetch(t + stride);
+    if (!kHold && k + 1 < rounds) fetch(t + stride, row + stride * p.d);
     // with one sum a row the next row's would write what this row's may still read
-    if (!(p.post && p.norm) && group > 32) __syncthreads();
+    if (!(POST && p.norm) && group > 32) __syncthreads();
   }
 }
 
-template <typename T, int CH, bool VEC, int MAXT>
+template <typename T, int CH, bool VEC, int MAXT, bool DROP, bool POST>
 __global__ void __launch_bounds__(MAXT, 512 / MAXT) residual_bwd_kernel(const DsaltResidualNormParams p, int group) {
   constexpr bool kHold = CH == 1;
-  __shared__ float red[2][3 * kMaxWarps];
+  __shared__ float4 red[2][kMaxWarps];
+  if (threadIdx.x < 2 * kMaxWarps) red[0][threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  __syncthreads();
   const int gid = threadIdx.x / group, lane = threadIdx.x - gid * group, per_cta = blockDim.x / group;
   const int64_t stride = (int64_t)gridDim.x * per_cta, first = (int64_t)blockIdx.x * per_cta + gid;
-  const int64_t rounds = (p.T - (int64_t)blockIdx.x * per_cta + stride - 1) / stride;
+  const int rounds = (int)((p.T - (int64_t)blockIdx.x * per_cta + stride - 1) / stride);
   Dropout dr;
   dr.init(p.seed, p.site, p.threshold);
   const T* Gt = reinterpret_cast<const T*>(p.gate);
   const bool with_h = p.norm && p.dh, full = p.gate_mode == DSALT_GATE_FULL;
-  const bool sums = with_h || p.post || p.gate_mode == DSALT_GATE_TOKEN;
+  const bool sums = with_h || POST || p.gate_mode == DSALT_GATE_TOKEN;
   const float inv_d = 1.f / (float)p.d;
   f2 wb[4], wn[4], a_branch[CH][4], a_norm[CH][4];
   if (kHold) column_factors<T>(p, dr, lane * 8, wb, wn);
@@ -233,13 +252,13 @@ __global__ void __launch_bounds__(MAXT, 512 / MAXT) residual_bwd_kernel(const Ds
     for (int j = 0; j < 4; ++j) a_branch[ch][j] = a_norm[ch][j] = dup(0.f);
   Raw<T, VEC> nx[CH], nf[CH], nd[CH], nh[CH];  // x', f, dx_new, dh
   float nr = 0.f, nrf = 1.f, ngt = 1.f;
-  auto fetch = [&](int64_t t) {
+  auto fetch = [&](int64_t t, int64_t row) {
     const bool on = t < p.T;
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (lane + ch * group) * 8;
       const bool in = on && c < p.d;
-      const int64_t at = t * p.d + c;
+      const int64_t at = row + c;
       auto one = [&](Raw<T, VEC>& raw, const void* q) {
         if (in && q) raw.load(reinterpret_cast<const T*>(q) + at, p.d - c);
         else raw.zero();
@@ -250,12 +269,13 @@ __global__ void __launch_bounds__(MAXT, 512 / MAXT) residual_bwd_kernel(const Ds
       one(nd[ch], p.dx_new);
     }
     nr = with_h && on ? __ldg(p.r + t) : 0.f;
-    nrf = p.post && on ? __ldg(p.rf + t) : 1.f;
+    nrf = POST && on ? __ldg(p.rf + t) : 1.f;
     ngt = p.gate_mode == DSALT_GATE_TOKEN && on ? to_f32<T>(Gt[t]) : 1.f;
   };
   int64_t t = first;
-  fetch(t);
-  for (int64_t k = 0; k < rounds; ++k, t += stride) {
+  int64_t row = t * p.d;  // index of the row's first element
+  fetch(t, row);
+  for (int k = 0; k < rounds; ++k, t += stride, row += stride * p.d) {
     const bool on = t < p.T;
     const float r = nr, rf = nrf, gt = ngt;
     const f2 r2 = dup(r);
@@ -265,14 +285,14 @@ __global__ void __launch_bounds__(MAXT, 512 / MAXT) residual_bwd_kernel(const Ds
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (lane + ch * group) * 8;
-      const int64_t at = t * p.d + c;
+      const int64_t at = row + c;
       f2 dh[4], g[4] = {dup(1.f), dup(1.f), dup(1.f), dup(1.f)};
       nx[ch].get(x[ch]);
       nf[ch].get(f[ch]);
       nd[ch].get(u[ch]);
       nh[ch].get(dh);
       if (!kHold) column_factors<T>(p, dr, c, wb, wn);
-      row_masks<VEC>(dr, at, m[ch]);
+      row_masks<VEC, DROP>(dr, at, m[ch]);
       if (full && on && c < p.d) {
         Raw<T, VEC> raw;
         raw.load(Gt + at, p.d - c);
@@ -286,14 +306,14 @@ __global__ void __launch_bounds__(MAXT, 512 / MAXT) residual_bwd_kernel(const Ds
         u[ch][j] = fma2(mul2(dh[j], wn[j]), r2, u[ch][j]);
         // κ: a dropped element passes nothing back, whatever f holds there
         f2 kf = and2(f[ch][j], m[ch][2 * j], m[ch][2 * j + 1]);
-        if (!p.post) f[ch][j] = kf;
+        if (!POST) f[ch][j] = kf;
         kf = mul2(kf, wb[j]);
         if (full) kf = mul2(kf, g[j]);
         s1 = fma2(kf, u[ch][j], s1);
         s2 = fma2(kf, x[ch][j], s2);
       }
     }
-    if (kHold && k + 1 < rounds) fetch(t + stride);
+    if (kHold && k + 1 < rounds) fetch(t + stride, row + stride * p.d);
     float s[3] = {sum8(s0), sum8(s1), sum8(s2)};
     if (sums) group_sum(s, group, red[k & 1]);
     const float e = r * r * r * (s[0] * inv_d);
@@ -304,7 +324,7 @@ __global__ void __launch_bounds__(MAXT, 512 / MAXT) residual_bwd_kernel(const Ds
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (lane + ch * group) * 8;
       if (!(on && c < p.d)) continue;
-      const int64_t at = t * p.d + c;
+      const int64_t at = row + c;
       if (!kHold) column_factors<T>(p, dr, c, wb, wn);
       Raw<T, VEC> out;
 #pragma unroll
@@ -334,14 +354,14 @@ __global__ void __launch_bounds__(MAXT, 512 / MAXT) residual_bwd_kernel(const Ds
           a_branch[ch][j] = fma2(mul2(G, f[ch][j]), al, a_branch[ch][j]);
         }
       }
-      if (p.post) {
+      if (POST) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) df[j] = fma2(f[ch][j], nm, df[j]);
       }
       out.set(df);
       out.store(reinterpret_cast<T*>(p.df) + at, p.d - c);
     }
-    if (!kHold && k + 1 < rounds) fetch(t + stride);
+    if (!kHold && k + 1 < rounds) fetch(t + stride, row + stride * p.d);
   }
   // this group's sums: partial row `first` of [groups][2][d] (Σ G⊙gate⊙f·rf where kept, Σ dh⊙x'·r)
   float* part = p.parts + first * 2 * p.d;
@@ -422,15 +442,19 @@ cudaError_t launch_v(const DsaltResidualNormParams& p, const Shape& s, bool bwd,
   int sms = 0;
   cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
-  if (!bwd) {
-    residual_fwd_kernel<T, CH, VEC, MAXT><<<(unsigned)ctas_of(p.T, s, kFwdThreads, sms), s.cta, 0, st>>>(p, s.group);
-    return cudaGetLastError();
-  }
-  const int64_t ctas = ctas_of(p.T, s, kBwdThreads, sms);
-  residual_bwd_kernel<T, CH, VEC, MAXT><<<(unsigned)ctas, s.cta, 0, st>>>(p, s.group);
+  const unsigned ctas = (unsigned)ctas_of(p.T, s, bwd ? kBwdThreads : kFwdThreads, sms);
+  auto run = [&](auto drop, auto post) {
+    if (bwd) residual_bwd_kernel<T, CH, VEC, MAXT, drop.value, post.value><<<ctas, s.cta, 0, st>>>(p, s.group);
+    else residual_fwd_kernel<T, CH, VEC, MAXT, drop.value, post.value><<<ctas, s.cta, 0, st>>>(p, s.group);
+  };
+  using Yes = std::true_type;
+  using No = std::false_type;
+  if (p.threshold > 0) p.post ? run(Yes(), Yes()) : run(Yes(), No());
+  else p.post ? run(No(), Yes()) : run(No(), No());
+  if (!bwd) return cudaGetLastError();
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   if (p.dscale || p.dpost || p.dnorm) {
-    residual_colsum_kernel<T><<<dim3((p.d + 31) / 32, p.dnorm ? 2 : 1), 1024, 0, st>>>(p, ctas * (s.cta / s.group));
+    residual_colsum_kernel<T><<<dim3((p.d + 31) / 32, p.dnorm ? 2 : 1), 1024, 0, st>>>(p, (int64_t)ctas * (s.cta / s.group));
     e = cudaGetLastError();
   }
   return e;
