@@ -10,11 +10,10 @@ namespace {
 constexpr int kThreads = 256;
 
 // A thread takes kBlocks blocks of eight elements (a counter's draws each), a CTA's
-// width apart, with their loads out before the first draw: one block a thread left the
-// memory waiting for loads (18 us for 16384 × 1024 bf16, DROP_US with kBlocks).
-constexpr int kBlocks = 4;
-
-template <typename T, bool VEC>
+// width apart, with their loads out before the first draw: four for tensors that fill
+// the device that way (16384 × 1024 bf16: 16 us, 18 with one), one for small tensors
+// (613 × 1001 fp32: 2.4 us, 4.2 with four).
+template <typename T, bool VEC, int kBlocks>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const DsaltDropoutParams p) {
   const int64_t first = ((int64_t)blockIdx.x * kBlocks * kThreads + threadIdx.x) * 8;
   Dropout dr;
@@ -51,14 +50,21 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DsaltDropoutPar
   }
 }
 
-template <typename T>
-cudaError_t launch_t(const DsaltDropoutParams& p, cudaStream_t st) {
+template <typename T, int kBlocks>
+cudaError_t launch_blocks(const DsaltDropoutParams& p, cudaStream_t st) {
   const bool vec = ((uintptr_t)p.x & 15) == 0 && ((uintptr_t)p.y & 15) == 0;
   const int64_t per_cta = 8 * kBlocks * kThreads;
   const unsigned grid = (unsigned)((p.n + per_cta - 1) / per_cta);
-  if (vec) dropout_kernel<T, true><<<grid, kThreads, 0, st>>>(p);
-  else dropout_kernel<T, false><<<grid, kThreads, 0, st>>>(p);
+  if (vec) dropout_kernel<T, true, kBlocks><<<grid, kThreads, 0, st>>>(p);
+  else dropout_kernel<T, false, kBlocks><<<grid, kThreads, 0, st>>>(p);
   return cudaGetLastError();
+}
+
+constexpr int64_t kLarge = (int64_t)8 * kThreads * 148 * 8;  // eight CTAs of one block for each of 148 SMs
+
+template <typename T>
+cudaError_t launch_t(const DsaltDropoutParams& p, cudaStream_t st) {
+  return p.n >= kLarge ? launch_blocks<T, 4>(p, st) : launch_blocks<T, 1>(p, st);
 }
 
 }  // namespace

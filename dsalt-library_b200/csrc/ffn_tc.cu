@@ -29,7 +29,7 @@
 //               a lane owns a row, so results are staged in shared memory and copied
 //               with row-contiguous 16-byte accesses (TMA stores of the same 64-byte
 //               rows shared the TMA unit with the operands' loads: hidden 175 us
-//               instead of HIDDEN_US at T = 16384, d = 1024, F = 2816)
+//               instead of 163 at T = 16384, d = 1024, F = 2816)
 // Every wait is bounded (sm100::mbar_wait).  Launches after the first of a call are
 // programmatic dependents: they set up their barriers and TMEM beside the end of the
 // launch before, and wait for its completion before they touch memory.
@@ -453,19 +453,20 @@ int tiles_of(const Jobs& jobs, int cols) {
   return (int)n;
 }
 
-// Tile columns (B rows of a pair) by estimated time: waves of tiles over the pairs ×
-// (K steps × a step's cycles + start and epilogue).  BN_COMMENT
+// Tile columns by estimated time: waves of tiles over the pairs × K steps × a step's
+// cycles, and the first loads and the last epilogue.  The numbers fit kernels measured
+// alone at T = 65 … 16384, d = 512 and 1024, e.g. (us with 256, 128, 64 columns) out at
+// T = 512, d = 1024, F = 2816: 18.8, 16.7, 16.2; hidden there: 15.5, 16.8, 19.8; out at
+// T = 16384: 75, 90, 165.
 int pick_bn(const Jobs& jobs, int steps, bool halves, bool b_mn, int pairs) {
-#ifdef FORCE_BN
-  return b_mn && FORCE_BN < 128 ? 128 : FORCE_BN;
-#endif
+  struct Width { int bn, step, ends; };
   int best = 256;
   int64_t best_cost = INT64_MAX;
-  for (const int bn : {256, 128, 64}) {
-    if (bn == 64 && b_mn) break;
-    const int64_t waves = (tiles_of(jobs, halves ? bn / 2 : bn) + pairs - 1) / pairs;
-    const int64_t cost = waves * ((int64_t)steps * (bn == 256 ? 640 : bn == 128 ? 400 : 300) + 2000);
-    if (cost < best_cost) best = bn, best_cost = cost;
+  for (const Width w : {Width{256, 680, 9500}, Width{128, 590, 4750}, Width{64, 550, 2850}}) {
+    if (w.bn == 64 && b_mn) break;  // an MN-major half tile is 64 columns at least
+    const int64_t waves = (tiles_of(jobs, halves ? w.bn / 2 : w.bn) + pairs - 1) / pairs;
+    const int64_t cost = waves * steps * w.step + w.ends;
+    if (cost < best_cost) best = w.bn, best_cost = cost;
   }
   return best;
 }

@@ -243,6 +243,8 @@ __global__ void __launch_bounds__(MAXT, 512 / MAXT) residual_bwd_kernel(const Ds
   const T* Gt = reinterpret_cast<const T*>(p.gate);
   const bool with_h = p.norm && p.dh, full = p.gate_mode == DSALT_GATE_FULL;
   const bool sums = with_h || POST || p.gate_mode == DSALT_GATE_TOKEN;
+  // without a norm, a scale or a gate on f nothing depends on its values
+  const void* f_rows = POST || p.dscale || p.gate_mode != DSALT_GATE_NONE ? p.f : nullptr;
   const float inv_d = 1.f / (float)p.d;
   f2 wb[4], wn[4], a_branch[CH][4], a_norm[CH][4];
   if (kHold) column_factors<T>(p, dr, lane * 8, wb, wn);
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(MAXT, 512 / MAXT) residual_bwd_kernel(const Ds
       };
       one(nx[ch], with_h ? p.x_new : nullptr);
       one(nh[ch], with_h ? p.dh : nullptr);
-      one(nf[ch], p.f);
+      one(nf[ch], f_rows);
       one(nd[ch], p.dx_new);
     }
     nr = with_h && on ? __ldg(p.r + t) : 0.f;

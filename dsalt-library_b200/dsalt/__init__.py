@@ -20,6 +20,10 @@ from dsalt.kernels import (  # noqa: F401
     soft_landmark_weights,
     HybridEnergyLandmarkSelector,
     LigerFusedLinearCrossEntropyFunction,
+    gated_ffn,
+    residual_norm,
+    counter_dropout,
+    new_dropout_seed,
 )
 
 __version__ = "1.0.0+b200"

@@ -6,6 +6,8 @@ Public names follow the reference's ``dsalt.kernels``.  The attention ops
 importing this package does not load the library, the first op call does (and
 raises if it is missing).  ``LigerFusedLinearCrossEntropyFunction`` (a Triton
 loss kernel, outside the attention path) is not provided and is ``None``.
+``gated_ffn``, ``residual_norm`` and ``counter_dropout`` are this build's own: the
+feed-forward half of a block.
 """
 
 from .RMSENorm import RMSENorm
@@ -26,6 +28,9 @@ from .landmark_tokens_ker import (
 from .dsalt_triton_bwd import dsalt_triton_backward
 from .dsalt_triton_attn import dsalt_triton_attention
 from .dsalt_triton_train import dsalt_triton_train_attention
+from .counter_dropout import counter_dropout, new_dropout_seed
+from .gated_ffn import gated_ffn
+from .residual_norm import residual_norm
 from .autotune import autotune_blocks, get_tuned_config
 
 LigerFusedLinearCrossEntropyFunction = None
@@ -49,4 +54,8 @@ __all__ = [
     "select_landmarks",
     "soft_landmark_weights",
     "HybridEnergyLandmarkSelector",
+    "gated_ffn",
+    "residual_norm",
+    "counter_dropout",
+    "new_dropout_seed",
 ]

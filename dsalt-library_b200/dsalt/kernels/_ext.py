@@ -280,6 +280,16 @@ def call_on(device: torch.device, name: str, params) -> None:
             call(name, params)
 
 
+def contiguous(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def first_derivative_only() -> None:
+    """For a backward whose launches autograd cannot differentiate: raise under ``create_graph``."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("this backward has no derivative of its own (create_graph is not supported)")
+
+
 def same_device(device: torch.device, **tensors) -> None:
     """Raise unless every given tensor (None is skipped) is on ``device``."""
     for name, t in tensors.items():

@@ -12,7 +12,6 @@ every replay.  ``site`` tells the places of one model apart that share a seed.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _ext
 
@@ -32,8 +31,14 @@ def check_seed(seed, site: int, device: torch.device) -> None:
     _ext.same_device(device, seed=seed)
 
 
+def new_dropout_seed(device: torch.device) -> torch.Tensor:
+    """A fresh seed from torch's generator of ``device`` (``torch.manual_seed`` governs it;
+    in a captured graph every replay draws another)."""
+    return torch.randint(0, 2 ** 62, (1,), dtype=torch.int64, device=device)
+
+
 def _launch(x: torch.Tensor, seed: torch.Tensor, site: int, threshold: int) -> torch.Tensor:
-    x = x.contiguous()
+    x = _ext.contiguous(x)
     y = torch.empty_like(x)
     p = _ext.DropoutParams(x=x.data_ptr(), y=y.data_ptr(), seed=seed.data_ptr(), n=x.numel(), site=site,
                            threshold=threshold, dtype=_ext.dtype_code(x.dtype))
@@ -48,11 +53,11 @@ class CounterDropoutFunction(torch.autograd.Function):
     def forward(ctx, x, seed, site: int, threshold: int):
         ctx.save_for_backward(seed)
         ctx.site, ctx.threshold = site, threshold
-        return _launch(x.detach(), seed, site, threshold)
+        return _launch(x, seed, site, threshold)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _ext.first_derivative_only()
         (seed,) = ctx.saved_tensors
         return _launch(dy, seed, ctx.site, ctx.threshold), None, None, None
 

@@ -17,7 +17,6 @@ kernel, with torch's rounding at every step.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _ext
 from .dsalt_cuda import device_status
@@ -29,11 +28,12 @@ def _operand(t: torch.Tensor, dtype: torch.dtype):
     """``(tensor, row stride)`` of a 2-D operand as the kernels read it: ``t`` itself when
     its rows are contiguous, 16-byte aligned and apart, else a copy that is."""
     rows, cols = t.shape
-    if t.dtype == dtype and t.stride(1) == 1 and t.data_ptr() % 16 == 0:
+    ld, step = t.stride()
+    if t.dtype == dtype and step == 1 and t.data_ptr() % 16 == 0:
+        if ld % 8 == 0 and ld >= cols:
+            return t, ld
         if rows == 1:
             return t, (cols + 7) // 8 * 8
-        if t.stride(0) % 8 == 0 and t.stride(0) >= cols:
-            return t, t.stride(0)
     ld = (cols + 7) // 8 * 8
     buf = torch.empty(rows, ld, dtype=dtype, device=t.device)
     buf[:, :cols].copy_(t)
@@ -53,9 +53,13 @@ def _forward(x2, wg, wu, wd, activation: int, dtype: torch.dtype, keep: bool):
     """``(y, h, a, b, ab)``; the last three, 16-bit words, only with ``keep``."""
     p = _params(x2, wg, wu, wd, activation, dtype)
     dev = x2[0].device
-    h, a, b, ab = (torch.empty(p.T, p.ld_f, dtype=dtype, device=dev) if i == 0 or keep else None for i in range(4))
+    h = torch.empty(p.T, p.ld_f, dtype=dtype, device=dev)
     y = torch.empty(p.T, p.d_out, dtype=dtype, device=dev)
-    p.h, p.a, p.b, p.ab, p.y = h.data_ptr(), _ext.ptr(a), _ext.ptr(b), _ext.ptr(ab), y.data_ptr()
+    p.h, p.y = h.data_ptr(), y.data_ptr()
+    a = b = ab = None
+    if keep:
+        a, b, ab = (torch.empty_like(h) for _ in range(3))
+        p.a, p.b, p.ab = a.data_ptr(), b.data_ptr(), ab.data_ptr()
     _ext.call_on(dev, "dsalt_gated_ffn_fwd", p)
     return y, h, a, b, ab
 
@@ -65,7 +69,7 @@ class GatedFFNFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation: int, dtype: torch.dtype):
-        ops = [_operand(t.detach(), dtype) for t in (x, w_gate, w_up, w_down)]
+        ops = [_operand(t, dtype) for t in (x, w_gate, w_up, w_down)]
         y, *kept = _forward(*ops, activation, dtype, True)
         ctx.save_for_backward(*(t for t, _ in ops), *kept)
         ctx.strides = [ld for _, ld in ops]
@@ -74,8 +78,8 @@ class GatedFFNFunction(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _ext.first_derivative_only()
         *ops, h, a, b, ab = ctx.saved_tensors
         dtype, dev = ctx.dtype, h.device
         p = _params(*zip(ops, ctx.strides), ctx.activation, dtype)
@@ -99,7 +103,7 @@ class GatedFFNFunction(torch.autograd.Function):
                     grads[1 + i] = torch.empty(shape, dtype=out, device=dev)
             p.dw_gate, p.dw_up, p.dw_down = (_ext.ptr(t) for t in grads[1:])
         _ext.call_on(dev, "dsalt_gated_ffn_bwd", p)
-        return (*(t if t is None else t.to(dt) for t, dt in zip(grads, ctx.dtypes)), None, None)
+        return (*(t if t is None or t.dtype == dt else t.to(dt) for t, dt in zip(grads, ctx.dtypes)), None, None)
 
 
 def _check(x, w_gate, w_up, w_down, activation):

@@ -7,8 +7,9 @@ block (``dsalt_residual_norm_fwd`` / ``_bwd`` in ``csrc/residual_norm.cu``).
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _ext
 from .counter_dropout import check_seed, drop_threshold
@@ -16,10 +17,20 @@ from .counter_dropout import check_seed, drop_threshold
 
 def _vectors(dtype: torch.dtype, *vs):
     """The given weight vectors as the kernels read them (all of ``dtype``, or all fp32) and which."""
-    given = [v for v in vs if v is not None]
-    f32 = any(v.dtype != dtype for v in given)
+    f32 = any(v is not None and v.dtype != dtype for v in vs)
     want = torch.float32 if f32 else dtype
-    return [None if v is None else v.detach().to(want).contiguous() for v in vs], f32
+    return [v if v is None or (v.dtype == want and v.is_contiguous()) else v.detach().to(want).contiguous()
+            for v in vs], f32
+
+
+@lru_cache(maxsize=1024)
+def _parts(T: int, d: int, device: int) -> int:
+    """Partial rows of the backward's scratch."""
+    with torch.cuda.device(device):
+        n = _ext.load().dsalt_residual_norm_parts(T, d)
+    if n < 0:
+        raise RuntimeError(f"dsalt_residual_norm_parts failed: {_ext.status_string(-n)}")
+    return n
 
 
 def _params(x_new, f, gate, vectors, f32, seed, eps, site, threshold, gate_mode):
@@ -49,8 +60,8 @@ class ResidualNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, f, post, scale, gate, norm, seed, eps, site, threshold, gate_mode):
-        x, f = x.detach().contiguous(), f.detach().contiguous()
-        g = None if gate is None else gate.detach().contiguous()
+        x, f = _ext.contiguous(x), _ext.contiguous(f)
+        g = None if gate is None else _ext.contiguous(gate)
         vectors, f32 = _vectors(f.dtype, post, scale, norm)
         x_new, h, rf, r = _forward(x, f, g, vectors, f32, seed, eps, site, threshold, gate_mode, True)
         ctx.save_for_backward(x_new, f, g, *vectors, seed, rf, r)
@@ -61,26 +72,23 @@ class ResidualNormFunction(torch.autograd.Function):
         return x_new if h is None else (x_new, h)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dx_new, dh=None):
+        _ext.first_derivative_only()
         x_new, f, gate, post, scale, norm, seed, rf, r = ctx.saved_tensors
         p = _params(x_new, f, gate, (post, scale, norm), ctx.f32, seed, *ctx.scalars)
-        dx_new, dh = (None if t is None else t.contiguous() for t in (dx_new, dh))
+        dx_new, dh = (None if t is None else _ext.contiguous(t) for t in (dx_new, dh))
         dx, df = torch.empty_like(f), torch.empty_like(f)
         dgate = None if gate is None else torch.empty_like(gate)
         need = (ctx.needs_input_grad[2], ctx.needs_input_grad[3], ctx.needs_input_grad[5])
         dpost, dscale, dnorm = (torch.empty_like(v) if v is not None and n else None
                                 for v, n in zip((post, scale, norm), need))
-        with torch.cuda.device(f.device):
-            n = _ext.load().dsalt_residual_norm_parts(p.T, p.d)
-        if n < 0:
-            raise RuntimeError(f"dsalt_residual_norm_parts failed: {_ext.status_string(-n)}")
-        parts = torch.empty(max(n, 1), 2, p.d, dtype=torch.float32, device=f.device)
+        parts = torch.empty(_parts(p.T, p.d, f.device.index), 2, p.d, dtype=torch.float32, device=f.device)
         p.rf, p.r, p.dx_new, p.dh = _ext.ptr(rf), _ext.ptr(r), _ext.ptr(dx_new), _ext.ptr(dh)
         p.dx, p.df, p.dgate, p.parts = dx.data_ptr(), df.data_ptr(), _ext.ptr(dgate), parts.data_ptr()
         p.dpost, p.dscale, p.dnorm = _ext.ptr(dpost), _ext.ptr(dscale), _ext.ptr(dnorm)
         _ext.call_on(f.device, "dsalt_residual_norm_bwd", p)
-        dpost, dscale, dnorm = (t if t is None else t.to(dt) for t, dt in zip((dpost, dscale, dnorm), ctx.dtypes))
+        if ctx.f32:
+            dpost, dscale, dnorm = (t if t is None else t.to(dt) for t, dt in zip((dpost, dscale, dnorm), ctx.dtypes))
         return dx, df, dpost, dscale, dgate, dnorm, None, None, None, None, None
 
 
@@ -136,8 +144,8 @@ def residual_norm(x: torch.Tensor, f: torch.Tensor, norm_weight: torch.Tensor | 
         x_new, h = out if norm_weight is not None else (out, None)
     else:
         vectors, f32 = _vectors(x.dtype, post_weight, scale, norm_weight)
-        g = None if gate is None else gate.contiguous()
-        x_new, h, _, _ = _forward(x2.contiguous(), f2.contiguous(), g, vectors, f32, seed, float(eps), site, threshold,
+        g = None if gate is None else _ext.contiguous(gate)
+        x_new, h, _, _ = _forward(_ext.contiguous(x2), _ext.contiguous(f2), g, vectors, f32, seed, float(eps), site, threshold,
                                   gate_mode, False)
     if x.dim() != 2:
         x_new, h = x_new.view(x.shape), None if h is None else h.view(x.shape)

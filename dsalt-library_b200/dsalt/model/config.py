@@ -9,7 +9,19 @@ from pathlib import Path
 
 @dataclass
 class DSALTConfig:
-    """Hyperparameters of :class:`~dsalt.model.dsalt_lm.DSALTLMHeadModel` (same fields as the reference)."""
+    """Hyperparameters of :class:`~dsalt.model.dsalt_lm.DSALTLMHeadModel`.
+
+    The reference's fields, then this build's own, which leave the reference's model as
+    it is unless they are set:
+
+    ``ffn_impl``         ``"gemm"``: library GEMMs around the activation kernel; ``"fused"``: the
+                         library's own kernels (``kernels/gated_ffn.py``) in 16-bit compute
+    ``ffn_activation``   ``"silu"``, ``"gelu"`` or ``"gelu_tanh"``
+    ``post_norm``        an RMSNorm on each branch's output before it is added
+    ``residual_scale``   a learned scale for each channel of a branch, with this start value
+    ``residual_gate``    a learned sigmoid gate for each token of a branch
+    ``counter_dropout``  dropout by ``kernels/counter_dropout.py``, fused into the residual adds
+    """
 
     vocab_size: int
     d_model: int
@@ -30,6 +42,12 @@ class DSALTConfig:
     lm_head_chunk_size: int = 2048
     loss_fn: str = "chunked"
     aux_loss_weight: float = 0.0
+    ffn_impl: str = "gemm"
+    ffn_activation: str = "silu"
+    post_norm: bool = False
+    residual_scale: float | None = None
+    residual_gate: bool = False
+    counter_dropout: bool = False
 
     def __post_init__(self) -> None:
         if self.d_model % self.n_heads != 0:
@@ -43,6 +61,10 @@ class DSALTConfig:
                              f"({self.n_kv_heads}) for grouped-query attention")
         if self.loss_fn not in ("auto", "chunked", "liger"):
             raise ValueError(f"loss_fn must be 'auto', 'chunked' or 'liger', got {self.loss_fn!r}")
+        if self.ffn_impl not in ("gemm", "fused"):
+            raise ValueError(f"ffn_impl must be 'gemm' or 'fused', got {self.ffn_impl!r}")
+        if self.ffn_activation not in ("silu", "gelu", "gelu_tanh"):
+            raise ValueError(f"ffn_activation must be 'silu', 'gelu' or 'gelu_tanh', got {self.ffn_activation!r}")
 
     def to_dict(self) -> dict:
         return asdict(self)

@@ -21,6 +21,7 @@ import torch.nn.functional as F
 
 from ..kernels.RMSENorm import RMSENorm
 from ..kernels import _ext
+from ..kernels.counter_dropout import counter_dropout, new_dropout_seed
 from ..kernels.fused_ce import fused_chunked_cross_entropy
 from ..modules.dsalt_transformer import DSALTTransformerBlock
 from .config import DSALTConfig
@@ -54,7 +55,9 @@ class DSALTLMHeadModel(nn.Module):
 
     def __init__(self, vocab_size, d_model, n_layers, n_heads, n_min, n_max, k_lmk, max_seq_len, d_ff=None,
                  dropout=0.0, yarn_scale=1.0, tie_weights=True, padding_idx=None, lm_head_chunk_size=2048,
-                 loss_fn="chunked", aux_loss_weight=0.0, n_kv_heads=None, qkv_bias=False, rope_base=10000.0):
+                 loss_fn="chunked", aux_loss_weight=0.0, n_kv_heads=None, qkv_bias=False, rope_base=10000.0,
+                 ffn_impl="gemm", ffn_activation="silu", post_norm=False, residual_scale=None, residual_gate=False,
+                 counter_dropout=False):
         super().__init__()
         assert loss_fn in _LOSS_FN, f"loss_fn must be one of {list(_LOSS_FN)}"
         self.d_model = d_model
@@ -69,10 +72,14 @@ class DSALTLMHeadModel(nn.Module):
             d_ff = ((hidden + 127) // 128) * 128
         self.embed_tokens = nn.Embedding(vocab_size, d_model, padding_idx=padding_idx)
         self.embed_dropout = nn.Dropout(dropout)
+        self.counter_dropout = counter_dropout
         self.layers = nn.ModuleList([
             DSALTTransformerBlock(d_model=d_model, n_heads=n_heads, n_min=n_min, n_max=n_max, k_lmk=k_lmk,
                                   max_seq_len=max_seq_len, d_ff=d_ff, dropout=dropout, yarn_scale=yarn_scale,
-                                  layer_idx=i, n_kv_heads=n_kv_heads, qkv_bias=qkv_bias, rope_base=rope_base)
+                                  layer_idx=i, n_kv_heads=n_kv_heads, qkv_bias=qkv_bias, rope_base=rope_base,
+                                  ffn_impl=ffn_impl, ffn_activation=ffn_activation, post_norm=post_norm,
+                                  residual_scale=residual_scale, residual_gate=residual_gate,
+                                  counter_dropout=counter_dropout)
             for i in range(n_layers)
         ])
         self.final_norm = RMSENorm(d_model)
@@ -142,7 +149,15 @@ class DSALTLMHeadModel(nn.Module):
                 padding_mask=None) -> dict:
         if max_seqlen is None:
             max_seqlen = input_ids.shape[-1]
-        x = self.embed_dropout(self.embed_tokens(input_ids))
+        x = self.embed_tokens(input_ids)
+        seed, options = None, {}
+        if self.counter_dropout and self.training and self.embed_dropout.p > 0:
+            # one seed a step; each place of the model draws at its own site
+            seed = new_dropout_seed(x.device)
+            options = {"dropout_seed": seed}
+            x = counter_dropout(x, self.embed_dropout.p, seed)
+        else:
+            x = self.embed_dropout(x)
         x = self._to_autocast_dtype(x)
         aux_loss = torch.zeros((), device=input_ids.device, dtype=x.dtype)
         rope_cs = cu_list = None
@@ -154,9 +169,14 @@ class DSALTLMHeadModel(nn.Module):
         for layer in self.layers:
             x, layer_aux, pending = layer(x, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen,
                                           gradient_checkpointing=gradient_checkpointing, rope_cs=rope_cs,
-                                          cu_list=cu_list, pending=pending, defer=True)
+                                          cu_list=cu_list, pending=pending, defer=True, **options)
             aux_loss = aux_loss + layer_aux
-        x = self.final_norm(x) if pending is None else self.final_norm.add_forward(x, pending)[1]
+        if pending is None:
+            x = self.final_norm(x)
+        elif callable(pending):  # a block's residual step
+            x = pending(x, self.final_norm)[1]
+        else:
+            x = self.final_norm.add_forward(x, pending)[1]
         if labels is not None:
             loss = self._compute_loss(x, labels) + self.aux_loss_weight * aux_loss
             return {"loss": loss, "logits": None, "aux_loss": aux_loss.detach()}
