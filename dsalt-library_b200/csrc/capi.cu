@@ -417,6 +417,7 @@ static int check_ffn(const DsaltGatedFfnParams* p, bool bwd) {
       {p->w_down, p->ld_wd, p->F, !bwd || hidden},
       {p->dy, p->ld_dy, p->d_out, bwd},
       {p->h, p->ld_f, p->F, !bwd || p->dw_down},
+      {p->h_lo, p->ld_f, p->F, !bwd && ffn_few_tokens(*p)},
       {p->a, p->ld_f, p->F, kept},
       {p->b, p->ld_f, p->F, kept},
       {p->ab, p->ld_f, p->F, kept},

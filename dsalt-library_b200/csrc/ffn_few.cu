@@ -11,16 +11,15 @@
 // bytes all the same.  Weights go from global memory straight to the fragments: a lane
 // reads 16 contiguous bytes of a row (8 consecutive k), and since a sum over k does not
 // care for its order, those 8 serve as the fragment's k of two MMA steps, in A and B
-// alike.  The second launch starts early (programmatic dependent launch): it fetches
+// alike.  The second product takes h as two 16-bit words, the rounded value and the
+// rounding's rest, at no cost beside the weights' bytes: y is off by its own rounding
+// only.  The second launch starts early (programmatic dependent launch): it fetches
 // its first weights before it waits for h.
 #include <algorithm>
 
 #include "ffn.cuh"
 #include "ffn_act.cuh"
 
-#ifndef FEW_MAX
-#define FEW_MAX 64
-#endif
 namespace dsalt {
 namespace ffn {
 namespace {
@@ -31,6 +30,7 @@ struct FewArgs {
   const uint16_t* w[2];  // [M, K] stride ld_w: gate and up, or down
   int64_t ld_w[2];
   const uint16_t* in;    // [T, K] stride ld_in
+  uint16_t* h_lo;        // what h's rounding leaves, rounded: written beside h, read with it
   int64_t ld_in;
   uint16_t* out;         // [T, M] stride ld_out: h, or y
   uint16_t *a, *b, *ab;  // with `out`'s stride, or null
@@ -40,23 +40,12 @@ struct FewArgs {
   bool bf16;
 };
 
-// 8 consecutive elements from k of a row of K (zeros past K; `on` false: all zeros).
-// RO: through the read-only path, for what no launch still running writes.
+// 8 consecutive elements, or zeros.  RO: through the read-only path, for what no launch
+// still running writes.
 template <bool RO>
-__device__ __forceinline__ uint4 load_k8(const uint16_t* row, int k, int K, bool on) {
+__device__ __forceinline__ uint4 load_k8(const uint16_t* p, bool on) {
   uint4 v = make_uint4(0, 0, 0, 0);
-  if (!on || k >= K) return v;
-  if (k + 8 <= K) {
-    const uint4* p = reinterpret_cast<const uint4*>(row + k);
-    return RO ? __ldg(p) : __ldcg(p);
-  }
-  uint16_t e[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) e[j] = k + j < K ? (RO ? __ldg(row + k + j) : __ldcg(row + k + j)) : (uint16_t)0;
-  v.x = e[0] | (uint32_t)e[1] << 16;
-  v.y = e[2] | (uint32_t)e[3] << 16;
-  v.z = e[4] | (uint32_t)e[5] << 16;
-  v.w = e[6] | (uint32_t)e[7] << 16;
+  if (on) v = RO ? __ldg(reinterpret_cast<const uint4*>(p)) : __ldcg(reinterpret_cast<const uint4*>(p));
   return v;
 }
 
@@ -64,10 +53,10 @@ template <bool BF16>
 __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   if constexpr (BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
@@ -101,8 +90,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) ffn_few_kernel(const FewArgs p
       for (int m = 0; m < NM; ++m)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int row = row0 + g + 8 * i;
-          wr[s][m][i] = load_k8<true>(p.w[m] + row * p.ld_w[m], (from + s) * kBlockK + 8 * q, p.K, row < p.M && from + s < kb_end);
+          const int row = row0 + g + 8 * i, k = (from + s) * kBlockK + 8 * q;
+          wr[s][m][i] = load_k8<true>(p.w[m] + row * p.ld_w[m] + k, row < p.M && from + s < kb_end && k < p.K);
         }
   };
   load_weights(kb);
@@ -111,22 +100,26 @@ __global__ void __launch_bounds__(kWarps * 32, 2) ffn_few_kernel(const FewArgs p
   while (kb < kb_end) {
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) {
-      if (kb + s >= kb_end) break;
       // h comes from the launch before, which was still running when this one began
-      uint4 x[NT];
+      auto products = [&](const uint16_t* in) {
+        uint4 x[NT];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int64_t t = t0 + n * 8 + g;
-        x[n] = load_k8<NM == 2>(p.in + t * p.ld_in, (kb + s) * kBlockK + 8 * q, p.K, t < p.T);
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int m = 0; m < NM; ++m) {
-          const uint4 lo = wr[s][m][0], hi = wr[s][m][1];
-          mma16816<BF16>(c[m][n], lo.x, hi.x, lo.y, hi.y, x[n].x, x[n].y);
-          mma16816<BF16>(c[m][n], lo.z, hi.z, lo.w, hi.w, x[n].z, x[n].w);
+        for (int n = 0; n < NT; ++n) {
+          const int64_t t = t0 + n * 8 + g;
+          const int k = (kb + s) * kBlockK + 8 * q;
+          x[n] = load_k8<NM == 2>(in + t * p.ld_in + k, t < p.T && kb + s < kb_end && k < p.K);
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int m = 0; m < NM; ++m) {
+            const uint4 lo = wr[s][m][0], hi = wr[s][m][1];
+            mma16816<BF16>(c[m][n], lo.x, hi.x, lo.y, hi.y, x[n].x, x[n].y);
+            mma16816<BF16>(c[m][n], lo.z, hi.z, lo.w, hi.w, x[n].z, x[n].w);
+          }
+      };
+      products(p.in);
+      if constexpr (NM == 1) products(p.h_lo);
     }
     kb += kAhead;
     if (kb < kb_end) load_weights(kb);
@@ -188,7 +181,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) ffn_few_kernel(const FewArgs p
         p.ab[at] = (uint16_t)(next8(a, b, a, b));
       }
     }
-    p.out[at] = (uint16_t)(sm100::pack2(result, result, BF16) & 0xffffu);
+    const uint32_t word = sm100::pack2(result, result, BF16);
+    p.out[at] = (uint16_t)(word & 0xffffu);
+    if constexpr (NM == 2) {
+      const float rest = result - (BF16 ? __uint_as_float(word << 16) : __half2float(__ushort_as_half((uint16_t)word)));
+      p.h_lo[at] = (uint16_t)(sm100::pack2(rest, rest, BF16) & 0xffffu);
+    }
   }
   if (p.split > 1) sm100::cluster_sync();  // no CTA leaves while its sums are read
 }
@@ -251,7 +249,9 @@ cudaError_t launch_tokens(const FewArgs& a, cudaStream_t st) {
 }  // namespace
 }  // namespace ffn
 
-bool ffn_few_tokens(const DsaltGatedFfnParams& p) { return p.T <= FEW_MAX; }
+bool ffn_few_tokens(const DsaltGatedFfnParams& p) {
+  return p.T <= DSALT_FFN_FEW_TOKENS && p.d % 8 == 0 && p.F % 8 == 0;  // whole 16-byte pieces of K
+}
 
 cudaError_t launch_ffn_few(const DsaltGatedFfnParams& p, cudaStream_t st) {
   using namespace ffn;
@@ -263,6 +263,7 @@ cudaError_t launch_ffn_few(const DsaltGatedFfnParams& p, cudaStream_t st) {
   a.in = (const uint16_t*)p.x;
   a.ld_in = p.ld_x;
   a.out = (uint16_t*)p.h;
+  a.h_lo = (uint16_t*)p.h_lo;
   a.a = (uint16_t*)p.a;
   a.b = (uint16_t*)p.b;
   a.ab = (uint16_t*)p.ab;

@@ -142,7 +142,8 @@ class GqaReduceParams(ctypes.Structure):
 
 class GatedFfnParams(ctypes.Structure):
     _fields_ = [("x", _c_void_p), ("w_gate", _c_void_p), ("w_up", _c_void_p), ("w_down", _c_void_p),
-                ("h", _c_void_p), ("a", _c_void_p), ("b", _c_void_p), ("ab", _c_void_p), ("y", _c_void_p),
+                ("h", _c_void_p), ("a", _c_void_p), ("b", _c_void_p), ("ab", _c_void_p), ("h_lo", _c_void_p),
+                ("y", _c_void_p),
                 ("dy", _c_void_p), ("dg", _c_void_p), ("du", _c_void_p), ("dx", _c_void_p), ("dw_gate", _c_void_p),
                 ("dw_up", _c_void_p), ("dw_down", _c_void_p), ("status", _c_void_p), ("T", _i64),
                 ("ld_x", _i64), ("ld_wg", _i64), ("ld_wu", _i64), ("ld_wd", _i64), ("ld_f", _i64), ("ld_dy", _i64),
@@ -165,6 +166,7 @@ class ResidualNormParams(ctypes.Structure):
                 ("w_f32", _i32)]
 
 
+FFN_FEW_TOKENS = 64  # DSALT_FFN_FEW_TOKENS
 GATE_NONE, GATE_TOKEN, GATE_FULL = 0, 1, 2  # DSALT_GATE_*
 RESIDUAL_MAX_D = 16384  # DSALT_RESIDUAL_MAX_D
 

@@ -8,7 +8,7 @@ needs gradients also keeps ``a = act(g)`` and ``b = u·act'(g)``, from which the
 backward forms ``du = dh·a`` and ``dg = dh·b`` in the epilogue of the product that
 makes ``dh``.  Results are rounded once from the fp32 sums; on the way only the
 operands of a further product are rounded to 16 bits, ``h``, ``dg`` and ``du``
-(``a`` and ``b`` are kept to 24 bits).
+(``a`` and ``b`` are kept to 24 bits, and ``h`` to two words in a forward of few tokens).
 
 ``swiglu_ffn`` computes the same block with library GEMMs around an activation
 kernel, with torch's rounding at every step.
@@ -43,22 +43,26 @@ def _operand(t: torch.Tensor, dtype: torch.dtype):
 def _params(x2, wg, wu, wd, activation: int, dtype: torch.dtype):
     (x_, ld_x), (wg_, ld_wg), (wu_, ld_wu), (wd_, ld_wd) = x2, wg, wu, wd
     F, d = wg_.shape
-    return _ext.GatedFfnParams(x=x_.data_ptr(), w_gate=wg_.data_ptr(), w_up=wu_.data_ptr(), w_down=wd_.data_ptr(),
-                               status=device_status(x_.device).data_ptr(), T=x_.shape[0], ld_x=ld_x, ld_wg=ld_wg,
-                               ld_wu=ld_wu, ld_wd=ld_wd, ld_f=(F + 7) // 8 * 8, d=d, F=F, d_out=wd_.shape[0],
-                               activation=activation, dtype=_ext.dtype_code(dtype))
+    p = _ext.GatedFfnParams(x_.data_ptr(), wg_.data_ptr(), wu_.data_ptr(), wd_.data_ptr())
+    p.status = device_status(x_.device).data_ptr()
+    p.T, p.d, p.F, p.d_out = x_.shape[0], d, F, wd_.shape[0]
+    p.ld_x, p.ld_wg, p.ld_wu, p.ld_wd, p.ld_f = ld_x, ld_wg, ld_wu, ld_wd, (F + 7) // 8 * 8
+    p.activation, p.dtype = activation, _ext.dtype_code(dtype)
+    return p
 
 
 def _forward(x2, wg, wu, wd, activation: int, dtype: torch.dtype, keep: bool):
     """``(y, h, a, b, ab)``; the last three, 16-bit words, only with ``keep``."""
     p = _params(x2, wg, wu, wd, activation, dtype)
-    dev = x2[0].device
-    h = torch.empty(p.T, p.ld_f, dtype=dtype, device=dev)
-    y = torch.empty(p.T, p.d_out, dtype=dtype, device=dev)
+    T, dev = p.T, x2[0].device
+    # few tokens: h's rounding rests beside it (scratch)
+    h = torch.empty(2 * T if T <= _ext.FFN_FEW_TOKENS else T, p.ld_f, dtype=dtype, device=dev)
+    y = torch.empty(T, p.d_out, dtype=dtype, device=dev)
     p.h, p.y = h.data_ptr(), y.data_ptr()
+    p.h_lo = h.data_ptr() + 2 * T * p.ld_f
     a = b = ab = None
     if keep:
-        a, b, ab = (torch.empty_like(h) for _ in range(3))
+        a, b, ab = (torch.empty(T, p.ld_f, dtype=dtype, device=dev) for _ in range(3))
         p.a, p.b, p.ab = a.data_ptr(), b.data_ptr(), ab.data_ptr()
     _ext.call_on(dev, "dsalt_gated_ffn_fwd", p)
     return y, h, a, b, ab
@@ -110,15 +114,16 @@ def _check(x, w_gate, w_up, w_down, activation):
     _ext.require_cuda(x, "x")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
-    if x.dim() == 0 or w_gate.dim() != 2 or w_up.dim() != 2 or w_down.dim() != 2:
+    xs, gs, us, ds = x.shape, w_gate.shape, w_up.shape, w_down.shape
+    if not xs or len(gs) != 2 or len(ds) != 2:
         raise ValueError("gated_ffn takes x [..., d], w_gate and w_up [F, d], w_down [d_out, F]")
-    F, d = w_gate.shape
-    if x.shape[-1] != d or w_up.shape != w_gate.shape or w_down.shape[1] != F:
-        raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, "
-                         f"w_up {tuple(w_up.shape)}, w_down {tuple(w_down.shape)}")
-    if F == 0 or d == 0 or w_down.shape[0] == 0:
+    if xs[-1] != gs[1] or us != gs or ds[1] != gs[0]:
+        raise ValueError(f"shapes do not fit: x {tuple(xs)}, w_gate {tuple(gs)}, w_up {tuple(us)}, w_down {tuple(ds)}")
+    if 0 in gs or ds[0] == 0:
         raise ValueError("gated_ffn needs widths of at least 1")
-    _ext.same_device(x.device, w_gate=w_gate, w_up=w_up, w_down=w_down)
+    dev = x.device
+    if w_gate.device != dev or w_up.device != dev or w_down.device != dev:
+        _ext.same_device(dev, w_gate=w_gate, w_up=w_up, w_down=w_down)
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
@@ -137,11 +142,13 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if dtype not in (torch.float16, torch.bfloat16):
         raise TypeError("gated_ffn computes in float16 or bfloat16: pass 16-bit tensors of one dtype, use autocast "
                         f"or give dtype (got x {x.dtype}, w_gate {w_gate.dtype}, dtype {dtype})")
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    flat = x.dim() == 2
+    x2 = x if flat else x.reshape(-1, x.shape[-1])
     act = ACTIVATIONS[activation]
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
                                     or w_down.requires_grad):
         y = GatedFFNFunction.apply(x2, w_gate, w_up, w_down, act, dtype)
     else:
-        y = _forward(*(_operand(t, dtype) for t in (x2, w_gate, w_up, w_down)), act, dtype, False)[0]
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])
+        y = _forward(_operand(x2, dtype), _operand(w_gate, dtype), _operand(w_up, dtype), _operand(w_down, dtype), act,
+                     dtype, False)[0]
+    return y if flat else y.view(*x.shape[:-1], y.shape[1])

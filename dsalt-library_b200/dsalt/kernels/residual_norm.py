@@ -34,22 +34,37 @@ def _parts(T: int, d: int, device: int) -> int:
 
 
 def _params(x_new, f, gate, vectors, f32, seed, eps, site, threshold, gate_mode):
+    p = _ext.ResidualNormParams(None, f.data_ptr())
     post, scale, norm = vectors
-    return _ext.ResidualNormParams(f=f.data_ptr(), gate=_ext.ptr(gate), post=_ext.ptr(post), scale=_ext.ptr(scale),
-                                   norm=_ext.ptr(norm), x_new=x_new.data_ptr(), seed=_ext.ptr(seed), T=f.shape[0],
-                                   d=f.shape[1], eps=eps, site=site, threshold=threshold, gate_mode=gate_mode,
-                                   dtype=_ext.dtype_code(f.dtype), w_f32=int(f32))
+    if gate is not None:
+        p.gate = gate.data_ptr()
+    if post is not None:
+        p.post = post.data_ptr()
+    if scale is not None:
+        p.scale = scale.data_ptr()
+    if norm is not None:
+        p.norm = norm.data_ptr()
+    if seed is not None:
+        p.seed = seed.data_ptr()
+    p.x_new, (p.T, p.d), p.eps = x_new.data_ptr(), f.shape, eps
+    p.site, p.threshold, p.gate_mode, p.dtype, p.w_f32 = site, threshold, gate_mode, _ext.dtype_code(f.dtype), f32
+    return p
 
 
 def _forward(x, f, gate, vectors, f32, seed, eps, site, threshold, gate_mode, keep: bool):
     """``(x_new, h, rf, r)``; the inverse root mean squares only with ``keep``."""
-    post, _, norm = vectors
-    x_new = torch.empty_like(f)
-    h = torch.empty_like(f) if norm is not None else None
+    x_new, h, rf, r = torch.empty_like(f), None, None, None
     p = _params(x_new, f, gate, vectors, f32, seed, eps, site, threshold, gate_mode)
-    rf = torch.empty(p.T, dtype=torch.float32, device=f.device) if keep and post is not None else None
-    r = torch.empty(p.T, dtype=torch.float32, device=f.device) if keep and norm is not None else None
-    p.x, p.h, p.rf, p.r = x.data_ptr(), _ext.ptr(h), _ext.ptr(rf), _ext.ptr(r)
+    p.x = x.data_ptr()
+    if vectors[2] is not None:
+        h = torch.empty_like(f)
+        p.h = h.data_ptr()
+        if keep:
+            r = torch.empty(p.T, dtype=torch.float32, device=f.device)
+            p.r = r.data_ptr()
+    if keep and vectors[0] is not None:
+        rf = torch.empty(p.T, dtype=torch.float32, device=f.device)
+        p.rf = rf.data_ptr()
     _ext.call_on(f.device, "dsalt_residual_norm_fwd", p)
     return x_new, h, rf, r
 

@@ -494,7 +494,9 @@ DSALT_API int dsalt_swiglu_bwd(const DsaltSwigluParams* p, void* stream);
 /* Gated feed-forward block, f16 / bf16, fp32 accumulation:
  *   g = x·Wgᵀ, u = x·Wuᵀ, h = act(g)⊙u, y = h·Wdᵀ
  * (dsalt/modules/dsalt_transformer.py:10-21 with act = silu).  Operands are row-major
- * with row strides ld_* and read in place.  The forward writes y, h (rounded once from
+ * with row strides ld_* and read in place.  Up to DSALT_FFN_FEW_TOKENS tokens,
+ * with d and F multiples of 8, the forward is a kernel of its own, whose second product
+ * takes h to two 16-bit words (h + h_lo) and is not off by h's rounding.  The forward writes y, h (rounded once from
  * fp32) and, with a, b and ab set, what a backward needs of g and u: a = act(g) and
  * b = u⊙act'(g) as the upper 24 bits of their fp32 values, the upper 16 in a and b,
  * the next 8 of each in the low and high byte of ab.  The backward forms, of
@@ -504,6 +506,7 @@ DSALT_API int dsalt_swiglu_bwd(const DsaltSwigluParams* p, void* stream);
  * dtype, or in fp32 with w_grad_f32.  Inputs and h, a, b, ab, dg, du: 16-byte aligned,
  * strides multiples of 8; in those five columns F up to the next multiple of 8 may be
  * written.  y, dx and the weight gradients are dense, of any alignment.      */
+#define DSALT_FFN_FEW_TOKENS 64
 enum { DSALT_ACT_SILU = 0, DSALT_ACT_GELU = 1, DSALT_ACT_GELU_TANH = 2 };
 typedef struct DsaltGatedFfnParams {
   const void* x;              /* [T, d] stride ld_x */
@@ -514,6 +517,7 @@ typedef struct DsaltGatedFfnParams {
   void* a;                    /* [T, F] 16-bit words, stride ld_f, or NULL (inference) */
   void* b;                    /* likewise */
   void* ab;                   /* likewise */
+  void* h_lo;                 /* [T, F] stride ld_f: scratch of that forward */
   void* y;                    /* [T, d_out] */
   const void* dy;             /* [T, d_out] stride ld_dy        (backward) */
   void* dg;                   /* [T, F] stride ld_f */

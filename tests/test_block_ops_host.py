@@ -37,19 +37,19 @@ def test_gated_ffn_entry_points_reject_bad_arguments():
     from dsalt.kernels import _ext
 
     def params(**kw):
-        base = dict(x=16, w_gate=16, w_up=16, w_down=16, h=16, y=16, dy=16, T=4, ld_x=64, ld_wg=64, ld_wu=64, ld_wd=96,
+        base = dict(x=16, w_gate=16, w_up=16, w_down=16, h=16, h_lo=16, y=16, dy=16, T=4, ld_x=64, ld_wg=64, ld_wu=64, ld_wd=96,
                     ld_f=96, ld_dy=64, d=64, F=96, d_out=64, dtype=_ext.BF16)
         return _ext.GatedFfnParams(**{**base, **kw})
 
     fwd, bwd = "dsalt_gated_ffn_fwd", "dsalt_gated_ffn_bwd"
     assert rc(fwd, params(dtype=_ext.F32)) == DT
     for bad in (dict(T=-1), dict(d=0), dict(F=0), dict(d_out=-8), dict(activation=3), dict(ld_x=56), dict(ld_x=68),
-                dict(ld_f=88), dict(ld_wd=90), dict(x=0), dict(w_up=0), dict(h=0), dict(y=0), dict(a=16), dict(a=16, b=16)):
+                dict(ld_f=88), dict(ld_wd=90), dict(x=0), dict(w_up=0), dict(h=0), dict(h_lo=0), dict(y=0), dict(a=16), dict(a=16, b=16)):
         assert rc(fwd, params(**bad)) == ARG, bad
     assert rc(fwd, params(x=24)) == ALIGN
     assert rc(fwd, params(T=(1 << 30) + 1)) == LARGE
     assert rc(fwd, params(T=1 << 30, F=1 << 20, ld_wd=1 << 20, ld_f=1 << 20)) == LARGE
-    assert rc(fwd, params(T=0, x=0, y=0)) == 0
+    assert rc(fwd, params(T=0, x=0, y=0, h_lo=0)) == 0
     kept = dict(a=16, b=16, ab=16, dg=16, du=16)
     assert rc(bwd, params(dx=16)) == ARG                       # nothing kept by the forward
     assert rc(bwd, params(dx=16, **{**kept, "du": 0})) == ARG
