@@ -417,7 +417,7 @@ static int check_ffn(const DsaltGatedFfnParams* p, bool bwd) {
       {p->w_down, p->ld_wd, p->F, !bwd || hidden},
       {p->dy, p->ld_dy, p->d_out, bwd},
       {p->h, p->ld_f, p->F, !bwd || p->dw_down},
-      {p->h_lo, p->ld_f, p->F, !bwd && ffn_few_tokens(*p)},
+      {p->h_lo, p->ld_f, p->F, !bwd && ffn_two_words(*p)},
       {p->a, p->ld_f, p->F, kept},
       {p->b, p->ld_f, p->F, kept},
       {p->ab, p->ld_f, p->F, kept},
@@ -439,7 +439,9 @@ int dsalt_gated_ffn_fwd(const DsaltGatedFfnParams* p, void* stream) {
   const int rc = check_ffn(p, false);
   if (rc != DSALT_OK || p->T == 0) return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  if (ffn_few_tokens(*p)) return status_of(launch_ffn_few(*p, st));
+  // ffn_few.cu reads whole 16-byte pieces of K
+  if (p->T <= kFewTokens && p->d % 8 == 0 && p->F % 8 == 0) return status_of(launch_ffn_few(*p, st));
+  if (p->T <= kMidTokens) return status_of(launch_ffn_mid(*p, st));
   cudaError_t e = launch_ffn_tc(FFN_HIDDEN, *p, false, st);
   if (e == cudaSuccess) e = launch_ffn_tc(FFN_OUT, *p, true, st);
   return status_of(e);

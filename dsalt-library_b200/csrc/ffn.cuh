@@ -8,7 +8,12 @@ enum FfnStage { FFN_HIDDEN = 0, FFN_OUT = 1, FFN_BWD_HIDDEN = 2, FFN_BWD_INPUT =
 // any number of tokens, tensor cores (ffn_tc.cu); early: the launch before it in the
 // stream is another of these stages, beside whose end it may start
 cudaError_t launch_ffn_tc(int stage, const DsaltGatedFfnParams& p, bool early, cudaStream_t st);
-// the forward for few tokens (ffn_few.cu): both stages, the second launched early
-bool ffn_few_tokens(const DsaltGatedFfnParams& p);
+// the forward for a handful of tokens (ffn_few.cu) and for up to kMidTokens (ffn_mid.cu):
+// both stages, the second launched early.  Up to DSALT_FFN_FEW_TOKENS tokens h is kept in
+// two words.  Measured (us, hidden + out in a graph, bf16, d = 1024, F = 2816): MEASURED
+constexpr int kFewTokens = 16, kMidTokens = 256;
 cudaError_t launch_ffn_few(const DsaltGatedFfnParams& p, cudaStream_t st);
+cudaError_t launch_ffn_mid(const DsaltGatedFfnParams& p, cudaStream_t st);
+// h_lo is used: up to DSALT_FFN_FEW_TOKENS tokens
+inline bool ffn_two_words(const DsaltGatedFfnParams& p) { return p.T <= DSALT_FFN_FEW_TOKENS; }
 }  // namespace dsalt

@@ -54,6 +54,10 @@ __device__ __forceinline__ void act_pair(float g, float& a, float& da) {
   }
 }
 
+__device__ __forceinline__ float2 unpack2(uint32_t w, bool bf16) {
+  if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
 // Upper 16 bits of fp32 x (low half) and y: the words of a and b.
 __device__ __forceinline__ uint32_t upper16(float x, float y) {
   return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);

@@ -1,4 +1,4 @@
-// Forward of the gated feed-forward block for few tokens (serving: one token a
+// Forward of the gated feed-forward block for up to 16 tokens (serving: one token a
 // sequence): g = x·Wgᵀ, u = x·Wuᵀ, h = act(g)⊙u, then y = h·Wdᵀ, as two launches.
 // Bound: the weights' bytes (3·d·F), and at these sizes the latency of getting them.
 //
@@ -6,7 +6,7 @@
 // warps, and over the CTAs of a cluster where there are too few rows to fill the
 // device; the partial sums are added in the order of K through shared memory, so
 // results do not change from run to run.  The products are mma.sync m16n8k16 with the
-// weight rows as M and up to 64 tokens as N: a tile of the 5th-generation pipe would
+// weight rows as M and 8 or 16 tokens as N: a tile of the 5th-generation pipe would
 // have 128 weight rows, a fifth of the SMs would get one, and it would wait for the
 // bytes all the same.  Weights go from global memory straight to the fragments: a lane
 // reads 16 contiguous bytes of a row (8 consecutive k), and since a sum over k does not
@@ -63,7 +63,7 @@ __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uin
 // NT: groups of 8 tokens of a CTA.  NM: weight matrices, 2 (gate and up) or 1 (down).
 template <int NT, int NM, bool BF16, int ACT>
 __global__ void __launch_bounds__(kWarps * 32, 2) ffn_few_kernel(const FewArgs p) {
-  constexpr int kAhead = NT < 8 ? 4 : 2;  // K blocks whose weights a warp requests at once
+  constexpr int kAhead = 4;  // K blocks whose weights a warp requests at once
   constexpr int kTok = NT * 8, kSums = NM * kRows * kTok;
   extern __shared__ float red[];  // [kWarps][NM][kRows][kTok], then the CTA's sums in the first
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
@@ -240,18 +240,11 @@ cudaError_t launch_type(const FewArgs& a, cudaStream_t st) {
 }
 template <int NM, int ACT>
 cudaError_t launch_tokens(const FewArgs& a, cudaStream_t st) {
-  if (a.T <= 8) return launch_type<1, NM, ACT>(a, st);
-  if (a.T <= 16) return launch_type<2, NM, ACT>(a, st);
-  if (a.T <= 32) return launch_type<4, NM, ACT>(a, st);
-  return launch_type<8, NM, ACT>(a, st);
+  return a.T <= 8 ? launch_type<1, NM, ACT>(a, st) : launch_type<2, NM, ACT>(a, st);
 }
 
 }  // namespace
 }  // namespace ffn
-
-bool ffn_few_tokens(const DsaltGatedFfnParams& p) {
-  return p.T <= DSALT_FFN_FEW_TOKENS && p.d % 8 == 0 && p.F % 8 == 0;  // whole 16-byte pieces of K
-}
 
 cudaError_t launch_ffn_few(const DsaltGatedFfnParams& p, cudaStream_t st) {
   using namespace ffn;

@@ -494,9 +494,9 @@ DSALT_API int dsalt_swiglu_bwd(const DsaltSwigluParams* p, void* stream);
 /* Gated feed-forward block, f16 / bf16, fp32 accumulation:
  *   g = x·Wgᵀ, u = x·Wuᵀ, h = act(g)⊙u, y = h·Wdᵀ
  * (dsalt/modules/dsalt_transformer.py:10-21 with act = silu).  Operands are row-major
- * with row strides ld_* and read in place.  Up to DSALT_FFN_FEW_TOKENS tokens,
- * with d and F multiples of 8, the forward is a kernel of its own, whose second product
- * takes h to two 16-bit words (h + h_lo) and is not off by h's rounding.  The forward writes y, h (rounded once from
+ * with row strides ld_* and read in place.  Up to DSALT_FFN_FEW_TOKENS tokens
+ * the second product takes h to two 16-bit words (h + h_lo) and is not off by h's
+ * rounding.  The forward writes y, h (rounded once from
  * fp32) and, with a, b and ab set, what a backward needs of g and u: a = act(g) and
  * b = u⊙act'(g) as the upper 24 bits of their fp32 values, the upper 16 in a and b,
  * the next 8 of each in the low and high byte of ab.  The backward forms, of

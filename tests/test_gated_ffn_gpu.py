@@ -56,8 +56,8 @@ def reference(x, wg, wu, wd, dy, act):
     # |act'| <= 1.13 and |act''| <= 1.1 for the three activations
     ea, eb = 1.13 * dg_ + fast * (a.abs() + 1e-3 * g.abs()), 1.1 * dg_ + fast * (1 + b.abs())
     h, eh = a * u, a.abs() * du_ + (u.abs() + du_) * ea
-    # up to 64 tokens, with whole 16-byte pieces, the second product takes h to two 16-bit words
-    eh1 = eh + e * e * h.abs() + tiny if T <= 64 and d % 8 == F % 8 == 0 else rounded(h, eh)[1]
+    # up to 64 tokens the second product takes h to two 16-bit words
+    eh1 = eh + e * e * h.abs() + tiny if T <= 64 else rounded(h, eh)[1]
     out = {"y": rounded(*mm(h, eh1, wd.t(), F))}
     h, eh = rounded(h, eh)
     if dy is None:
@@ -97,7 +97,8 @@ def inputs(T, d, F, d_out, dtype, seed=0, grad=True):
     return [t.requires_grad_(grad) for t in ts] + [n(T, d_out)]
 
 
-SIZES = [(1, 8, 8, 8), (1, 64, 96, 64), (2, 1, 1, 1), (3, 17, 5, 9), (5, 40, 72, 40), (17, 72, 136, 24), (64, 256, 512, 256),
+SIZES = [(16, 264, 72, 1000), (17, 1024, 200, 8), (31, 65, 130, 67), (33, 520, 1368, 520), (64, 72, 40, 136), (65, 200, 264, 136),
+         (128, 264, 520, 264), (200, 129, 63, 258), (256, 512, 1408, 512), (1, 8, 8, 8), (1, 64, 96, 64), (2, 1, 1, 1), (3, 17, 5, 9), (5, 40, 72, 40), (17, 72, 136, 24), (64, 256, 512, 256),
          (127, 64, 128, 64), (129, 200, 264, 136), (300, 96, 1000, 96), (257, 63, 129, 65), (640, 512, 1408, 512)]
 
 
