@@ -164,20 +164,26 @@ __global__ void __launch_bounds__(kThreads) ffn_mid_kernel(const __grid_constant
   const int quads = p.rows / 4;
   const uint32_t base = smem_u32(sums);
   uint32_t peer[kMaxSplit];
-  for (int s = 0; s < p.split; ++s) peer[s] = p.split > 1 ? map_rank(base, s) : base;
+#pragma unroll
+  for (int s = 0; s < kMaxSplit; ++s) peer[s] = p.split > 1 ? map_rank(base, min(s, p.split - 1)) : base;
   for (int i = tid; i < (t_end - (int)rank * share) * quads; i += kThreads) {
     const int t = (int)rank * share + i / quads, r = i % quads * 4, row = row0 + r;
     if (row >= p.M) continue;
-    auto total = [&](int from) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int s = 0; s < p.split; ++s) {
-        const float4 x = cluster_load4(peer[s] + (uint32_t)(t * 128 + from + r) * 4);
-        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+    // every load on its way before the first sum; added in the order of K
+    float4 xg[kMaxSplit], xu[kMaxSplit];
+#pragma unroll
+    for (int s = 0; s < kMaxSplit; ++s)
+      if (s < p.split) {
+        xg[s] = cluster_load4(peer[s] + (uint32_t)(t * 128 + r) * 4);
+        if (HIDDEN) xu[s] = cluster_load4(peer[s] + (uint32_t)(t * 128 + 64 + r) * 4);
       }
-      return v;
-    };
-    const float4 g4 = total(0);
+    float4 g4 = xg[0], u4 = xu[0];
+#pragma unroll
+    for (int s = 1; s < kMaxSplit; ++s)
+      if (s < p.split) {
+        g4.x += xg[s].x; g4.y += xg[s].y; g4.z += xg[s].z; g4.w += xg[s].w;
+        if (HIDDEN) u4.x += xu[s].x, u4.y += xu[s].y, u4.z += xu[s].z, u4.w += xu[s].w;
+      }
     float v[4] = {g4.x, g4.y, g4.z, g4.w};
     const int64_t at = (int64_t)(t0 + t) * p.ld_out + row;
     auto put = [&](uint16_t* dst, uint32_t lo, uint32_t hi) {
@@ -189,7 +195,6 @@ __global__ void __launch_bounds__(kThreads) ffn_mid_kernel(const __grid_constant
       }
     };
     if constexpr (HIDDEN) {
-      const float4 u4 = total(64);
       const float u[4] = {u4.x, u4.y, u4.z, u4.w};
       float a[4], b[4];
 #pragma unroll
