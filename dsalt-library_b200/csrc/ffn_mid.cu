@@ -1,5 +1,5 @@
 // Forward of the gated feed-forward block for a batch of tokens that is still short of
-// a tile of ffn_tc.cu (17 to 256: a step of many sequences, a short prompt), as two
+// a tile of ffn_tc.cu (17 to 384: a step of many sequences, a short prompt), as two
 // launches.  Bound: the weights' bytes and the latency of the way to them; with tiles of
 // 256 tokens × 128 features a handful of SM pairs would fetch all weights.
 //
