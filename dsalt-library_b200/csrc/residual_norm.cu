@@ -14,7 +14,7 @@
 // 32 lanes of a warp up to d = 256, else a whole CTA (of one, two or four chunks of
 // columns a thread).  A group walks rows of the grid's stride with the
 // next row's loads on their way, its weights and column sums in registers; the sums of
-// a group go to one partial row and a second kernel adds the partial rows in order.
+// a CTA go to one partial row and a second kernel adds the partial rows in order.
 //
 // The backward needs Σ dh⊙norm⊙x' before G, and Σ κ⊙G with κ = D⊙scale⊙gate⊙post⊙f
 // (for df and a token's dgate; κ there without the token's gate) after it.  G = u − e·x' with u = dx_new + r·dh⊙norm and
@@ -378,8 +378,28 @@ __global__ void __launch_bounds__(MAXT, CH == 1 ? 512 / MAXT : 1) residual_bwd_k
     }
     if (!kHold && k + 1 < rounds) fetch(t + stride, row + stride * p.d);
   }
-  // this group's sums: partial row `first` of [groups][2][d] (Σ G⊙gate⊙f·rf where kept, Σ dh⊙x'·r)
-  float* part = p.parts + first * 2 * p.d;
+  // this CTA's sums: partial row blockIdx.x of [CTAs][2][d] (Σ G⊙gate⊙f·rf where kept,
+  // Σ dh⊙x'·r); several groups' sums are added in order first
+  float* part = p.parts + (int64_t)blockIdx.x * 2 * p.d;
+  if (per_cta > 1) {
+    __shared__ float group_sums[CH == 1 && MAXT == 256 ? 2 * kSmallThreads * 8 : 1];
+    if constexpr (CH == 1 && MAXT == 256) {
+      float* mine = group_sums + gid * 2 * group * 8 + lane * 8;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        unpair(a_branch[0][j], mine[2 * j], mine[2 * j + 1]);
+        unpair(a_norm[0][j], mine[group * 8 + 2 * j], mine[group * 8 + 2 * j + 1]);
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < 2 * p.d; i += blockDim.x) {
+        const int at = i < p.d ? i : group * 8 + i - p.d;
+        float v = 0.f;
+        for (int g = 0; g < per_cta; ++g) v += group_sums[g * 2 * group * 8 + at];
+        part[i] = v;
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int ch = 0; ch < CH; ++ch) {
     const int c = (lane + ch * group) * 8;
@@ -468,7 +488,7 @@ cudaError_t launch_v(const DsaltResidualNormParams& p, const Shape& s, bool bwd,
   if (!bwd) return cudaGetLastError();
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   if (p.dscale || p.dpost || p.dnorm) {
-    residual_colsum_kernel<T><<<dim3((p.d + 31) / 32, p.dnorm ? 2 : 1), 1024, 0, st>>>(p, (int64_t)ctas * (s.cta / s.group));
+    residual_colsum_kernel<T><<<dim3((p.d + 31) / 32, p.dnorm ? 2 : 1), 1024, 0, st>>>(p, ctas);
     e = cudaGetLastError();
   }
   return e;
@@ -500,7 +520,7 @@ cudaError_t residual_norm_parts(int64_t T, int d, int* out) {
   *out = 0;
   for (const bool vec : {false, true}) {
     const Shape s = shape_of(d, vec);
-    *out = std::max(*out, (int)ctas_of(T, s, true, sms) * (s.cta / s.group));
+    *out = std::max(*out, (int)ctas_of(T, s, true, sms));
   }
   return cudaSuccess;
 }
