@@ -59,8 +59,9 @@ KERNELS_PER_CALL = {"dsalt_build_schedule": 2, "dsalt_gather_landmarks": 1, "dsa
 # pass and the fix-up kernel accompany)
 NCU_TRAFFIC_BYTES = {"config2": {"dsalt_attn_fwd": 301239808, "dsalt_attn_bwd_dkdv": 687554688,
                                  "dsalt_attn_bwd_dq": 515452800}}
-# digest of csrc/ (kernel_source_digest) when that capture was taken; other sources -> traffic null
-NCU_TRAFFIC_SRC = "232497833c0a8d95"
+# digest of the attention sources (kernel_source_digest) when that capture was taken; other
+# sources -> traffic null
+NCU_TRAFFIC_SRC = "3ab6bdd212f34c1f"
 CLOCK_REASONS = {0x1: "gpu_idle", 0x2: "applications_clocks_setting", 0x4: "sw_power_cap",
                  0x8: "hw_slowdown", 0x10: "sync_boost", 0x20: "sw_thermal_slowdown",
                  0x40: "hw_thermal_slowdown", 0x80: "hw_power_brake_slowdown", 0x100: "display_clock_setting"}
@@ -1085,9 +1086,11 @@ def ncu_traffic(workload, kernel, world):
 
 
 def kernel_source_digest() -> str:
+    """Digest of the attention kernels' sources and the headers they include."""
     import hashlib
     h = hashlib.sha256()
-    for f in sorted((ROOT / "dsalt-library_b200" / "csrc").glob("*.cu*")):
+    csrc = ROOT / "dsalt-library_b200" / "csrc"
+    for f in sorted([*csrc.glob("attn_*.cu"), csrc / "common.cuh", csrc / "sm100.cuh"]):
         h.update(f.name.encode())
         h.update(f.read_bytes())
     return h.hexdigest()[:16]
