@@ -38,6 +38,17 @@ def device_status(device: torch.device) -> torch.Tensor:
     return st
 
 
+def device_status_ptr(device: torch.device) -> int:
+    """Address of the device's status word; 0 (kernels then report nothing) where it would have
+    to be made inside a graph capture, whose memory and zero fill belong to the graph."""
+    st = _STATUS.get(("cuda", device.index))
+    if st is None:
+        if torch.cuda.is_current_stream_capturing():
+            return 0
+        st = device_status(device)
+    return st.data_ptr()
+
+
 def check_device_status(device: torch.device, reset: bool = True) -> int:
     """Read (and optionally clear) the device status word; raise on a fault bit."""
     st = device_status(device)

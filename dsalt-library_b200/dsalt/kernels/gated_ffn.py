@@ -19,7 +19,7 @@ from __future__ import annotations
 import torch
 
 from . import _ext
-from .dsalt_cuda import device_status
+from .dsalt_cuda import device_status_ptr
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}  # DSALT_ACT_*
 
@@ -44,7 +44,7 @@ def _params(x2, wg, wu, wd, activation: int, dtype: torch.dtype):
     (x_, ld_x), (wg_, ld_wg), (wu_, ld_wu), (wd_, ld_wd) = x2, wg, wu, wd
     F, d = wg_.shape
     p = _ext.GatedFfnParams(x_.data_ptr(), wg_.data_ptr(), wu_.data_ptr(), wd_.data_ptr())
-    p.status = device_status(x_.device).data_ptr()
+    p.status = device_status_ptr(x_.device)
     p.T, p.d, p.F, p.d_out = x_.shape[0], d, F, wd_.shape[0]
     p.ld_x, p.ld_wg, p.ld_wu, p.ld_wd, p.ld_f = ld_x, ld_wg, ld_wu, ld_wd, (F + 7) // 8 * 8
     p.activation, p.dtype = activation, _ext.dtype_code(dtype)

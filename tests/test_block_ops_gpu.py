@@ -169,3 +169,62 @@ def test_first_backward_of_a_process_may_be_a_gated_ffn():
     t.start()
     t.join()
     assert len(got) == 1 and all(torch.isfinite(g).all() for g in got[0])
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    """A captured call finds no status word yet: it makes none that would live in the graph."""
+    from dsalt import gated_ffn
+    from dsalt.kernels import dsalt_cuda
+    ts = [torch.randn(*s, device="cuda").bfloat16() for s in ((400, 64), (96, 64), (96, 64), (64, 96))]
+    ref = gated_ffn(*ts)
+    saved = dict(dsalt_cuda._STATUS)
+    dsalt_cuda._STATUS.clear()
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = gated_ffn(*ts)
+        assert not dsalt_cuda._STATUS
+    finally:
+        dsalt_cuda._STATUS.update(saved)
+    graph.replay()
+    assert torch.equal(y, ref)
+    dsalt_cuda.check_device_status(ref.device)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^32 elements: the last rows equal the same rows of a small call (rows do not
+    depend on one another; the feed-forward sums have one order in both tilings)."""
+    from dsalt import gated_ffn, residual_norm
+    d, T, n = 1024, (1 << 22) + 5, 700
+    x, f = (torch.zeros(T, d, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    x[-n:], f[-n:] = torch.randn(n, d, device="cuda"), torch.randn(n, d, device="cuda")
+    w = torch.rand(d, device="cuda") + 0.5
+    big, small = residual_norm(x, f, w, post_weight=w), residual_norm(x[-n:], f[-n:], w, post_weight=w)
+    assert all(torch.equal(a[-n:], b) for a, b in zip(big, small))
+    del big, small, f
+    x = x.view(-1, 64)[-(1 << 21) - 3:]                      # 2^21 tokens of 64, 2^32.5 hidden values
+    ws = [torch.randn(2816, 64, device="cuda").bfloat16() / 8 for _ in range(2)] + [torch.randn(64, 2816, device="cuda").bfloat16() / 50]
+    with torch.no_grad():
+        y = gated_ffn(x, *ws)
+        assert torch.equal(y[-n:], gated_ffn(x[-n:], *ws))
+
+
+def test_gradients_past_32_bits():
+    """The backward's offsets too: gradients of the last rows, and the weight's from them alone."""
+    from dsalt import gated_ffn
+    T, n = (1 << 20) + 37, 500
+    x = torch.zeros(T, 64, device="cuda", dtype=torch.bfloat16)
+    x[-n:] = torch.randn(n, 64, device="cuda")
+    ws = [torch.randn(s, device="cuda").bfloat16() / 8 for s in ((4224, 64), (4224, 64), (64, 4224))]
+    dy = torch.zeros(T, 64, device="cuda", dtype=torch.bfloat16)
+    dy[-n:] = torch.randn(n, 64, device="cuda")
+
+    def grads(x, dy):
+        ts = [t.detach().requires_grad_(True) for t in (x, *ws)]
+        return torch.autograd.grad(gated_ffn(*ts), ts, dy)
+
+    big, small = grads(x, dy), grads(x[-n:], dy[-n:])
+    assert torch.equal(big[0][-n:], small[0]) and not big[0][:-n].any()
+    for a, b in zip(big[1:], small[1:]):  # the same terms at other places of the fp32 sum, one rounding
+        mag = b.float().abs().max()
+        assert ((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 2.0 ** -10 * mag).all()
