@@ -59,7 +59,11 @@ struct Cfg {
   static constexpr int kThreads = (2 + kEpiWarps) * 32;
   static constexpr int kColStep = kEpiWarps / 4 * 32;           // columns from a warp's chunk to its next
   static constexpr int kBoxes = EPI == EPI_DHIDDEN ? 3 : 2;     // staged boxes of a warp
-  static constexpr int kStages = EPI == EPI_DHIDDEN ? 4 : 6;
+  static constexpr int kStages = EPI == EPI_DHIDDEN || BN == 512 ? 4 : 6;
+  // 512 columns fill TMEM with one accumulator: the epilogue waits beside nothing, which
+  // only a long K forgives
+  static constexpr int kAcc = BN == 512 ? 1 : 2;
+  static constexpr int kMmaN = BN == 512 ? 256 : BN, kMmas = BN / kMmaN;
   static constexpr int FULL = 0, EMPTY = kStages, ACC_FULL = 2 * kStages, ACC_EMPTY = ACC_FULL + 2,
                        FINAL = ACC_EMPTY + 2, NB = FINAL + 1;
   struct alignas(1024) Smem {
@@ -198,7 +202,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI>::kThrea
     fence_mbar_init();
     sm.abort_flag = 0;
   }
-  if (warp == 1) tmem_alloc_pair(smem_u32(&sm.tmem_base), 2 * BN);
+  if (warp == 1) tmem_alloc_pair(smem_u32(&sm.tmem_base), C::kAcc * BN);
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // both CTAs' barriers exist before either signals the other's
@@ -230,8 +234,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI>::kThrea
           load_piece<AMN, 128>(base, &a.ma[im], full, tl.m0 + 128 * rank, k0);
           if constexpr (EPI == EPI_HIDDEN)  // the same columns of gate (leader) and up (its peer)
             load_piece<BMN, BN / 2>(base + kPiece, &a.mb[rank], full, tl.nt * (BN / 2), k0);
-          else
-            load_piece<BMN, BN / 2>(base + kPiece, &a.mb[im], full, tl.nt * BN + (BN / 2) * rank, k0);
+          else  // this CTA's half of each MMA's columns
+#pragma unroll
+            for (int j = 0; j < C::kMmas; ++j)
+              load_piece<BMN, C::kMmaN / 2>(base + kPiece + j * C::kMmaN / 2 * BK * 2, &a.mb[im], full,
+                                            tl.nt * BN + j * C::kMmaN + (C::kMmaN / 2) * (int)rank, k0);
         }
       }
       // the last products have read this CTA's shared memory, and their signals have come
@@ -240,12 +247,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI>::kThrea
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0 && rank == 0) {
-      const uint32_t idesc = idesc_f16(a.bf16, BM, BN, AMN, BMN);
+      const uint32_t idesc = idesc_f16(a.bf16, BM, C::kMmaN, AMN, BMN);
       int g = 0, li = 0;
       bool ok = true;
       for (int t = t0; ok && t < a.n_tiles; t += t_step, ++li) {
-        const int acc = li & 1;
-        if (li >= 2) ok = mbar_wait(bar[C::ACC_EMPTY + acc], ((li >> 1) - 1) & 1, abort_flag, a.status);
+        const int acc = li % C::kAcc;
+        if (li >= C::kAcc) ok = mbar_wait(bar[C::ACC_EMPTY + acc], (li / C::kAcc - 1) & 1, abort_flag, a.status);
         tc_fence_after();
         for (int s = 0; ok && s < steps; ++s, ++g) {
           const int st = g % kStages;
@@ -257,8 +264,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI>::kThrea
           const uint32_t base = smem_u32(sm.ring[st]);
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk)
-            mma_f16_pair(tmem + acc * BN, piece_desc<AMN>(base, kk), piece_desc<BMN>(base + kPiece, kk), idesc,
-                         (s > 0 || kk > 0) ? 1u : 0u);
+#pragma unroll
+            for (int j = 0; j < C::kMmas; ++j)
+              mma_f16_pair(tmem + acc * BN + j * C::kMmaN, piece_desc<AMN>(base, kk),
+                           piece_desc<BMN>(base + kPiece + j * C::kMmaN / 2 * BK * 2, kk), idesc, (s > 0 || kk > 0) ? 1u : 0u);
           mma_commit_pair(bar[C::EMPTY + st]);
         }
         if (ok) mma_commit_pair(bar[C::ACC_FULL + acc]);
@@ -277,7 +286,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI>::kThrea
     for (int t = t0; t < a.n_tiles; t += t_step, ++li) {
       const Tile tl = decode(a, t);
       const Problem& pr = a.prob[tl.prob];
-      const int acc = li & 1;
+      const int acc = li % C::kAcc;
       const int row0 = tl.m0 + 128 * (int)rank + 32 * q4, rows = pr.M - row0;  // rows of this warp (may be <= 0)
       const int col0 = tl.nt * kCols, cols = pr.N - col0;
       const int64_t at = EPI == EPI_STORE ? row0 * pr.ld_out + col0 : row0 * a.ld_f + col0;
@@ -288,7 +297,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI>::kThrea
       };
       if constexpr (EPI == EPI_DHIDDEN)  // on the way while the products finish
         if (cg * 32 < kCols) load_ab(cg * 32);
-      if (!__all_sync(0xffffffffu, mbar_wait(bar[C::ACC_FULL + acc], (li >> 1) & 1, abort_flag, a.status))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(bar[C::ACC_FULL + acc], (li / C::kAcc) & 1, abort_flag, a.status))) break;
       tc_fence_after();
       const uint32_t tacc = tmem + acc * BN + lane_addr;
       auto release = [&]() {  // this warp has read its part: the products may reuse the accumulator
@@ -411,7 +420,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI>::kThrea
   __syncthreads();
   cluster_sync();  // the peer's products, copies and signals for this CTA are done
   tc_fence_after();
-  if (warp == 1) tmem_dealloc_pair(tmem, 2 * BN);
+  if (warp == 1) tmem_dealloc_pair(tmem, C::kAcc * BN);
 }
 
 // --------------------------------------------------------------------- host
@@ -458,10 +467,18 @@ int tiles_of(const Jobs& jobs, int cols) {
 // alone at T = 65 … 16384, d = 512 and 1024, e.g. (us with 256, 128, 64 columns) out at
 // T = 512, d = 1024, F = 2816: 18.8, 16.7, 16.2; hidden there: 15.5, 16.8, 19.8; out at
 // T = 16384: 75, 90, 165.
-int pick_bn(const Jobs& jobs, int steps, bool halves, bool b_mn, int pairs) {
+int pick_bn(const Jobs& jobs, int steps, bool halves, bool b_mn, int pairs, bool wide = false) {
   struct Width { int bn, step, ends; };
   int best = 256;
   int64_t best_cost = INT64_MAX;
+  // 512 columns: a quarter less to fetch for the same products, one accumulator (us with
+  // 256 and 512: the weight gradients at T = 16384, d = 1024, F = 2816: 246, 224; at
+  // T = 8192, d = 2048, F = 5632: 489, 452)
+  if (wide) {
+    const int64_t waves = (tiles_of(jobs, 512) + pairs - 1) / pairs;
+    best = 512;
+    best_cost = waves * (steps * 1150 + 16000);
+  }
   for (const Width w : {Width{256, 680, 9500}, Width{128, 590, 4750}, Width{64, 550, 2850}}) {
     if (w.bn == 64 && b_mn) break;  // an MN-major half tile is 64 columns at least
     const int64_t waves = (tiles_of(jobs, halves ? w.bn / 2 : w.bn) + pairs - 1) / pairs;
@@ -506,6 +523,8 @@ cudaError_t launch_bn(const Args& a, int pairs, cudaStream_t st) {
 template <bool AMN, bool BMN, int EPI, int ACT = 0>
 cudaError_t launch(const Args& a, int bn, int pairs, cudaStream_t st) {
   if (bn == 256) return launch_bn<AMN, BMN, EPI, 256, ACT>(a, pairs, st);
+  if constexpr (AMN)
+    if (bn == 512) return launch_bn<AMN, BMN, EPI, 512, ACT>(a, pairs, st);
   if constexpr (!BMN)
     if (bn == 64) return launch_bn<AMN, BMN, EPI, 64, ACT>(a, pairs, st);
   return launch_bn<AMN, BMN, EPI, 128, ACT>(a, pairs, st);
@@ -620,7 +639,7 @@ cudaError_t launch_ffn_tc(int stage, const DsaltGatedFfnParams& p, bool early, c
       }
       if (n == 0) return cudaSuccess;
       const Jobs jobs = {job, n};
-      const int bn = pick_bn(jobs, steps(a.K), false, true, pairs);
+      const int bn = pick_bn(jobs, steps(a.K), false, true, pairs, true);
       set_jobs(a, jobs, bn);
       set_out(a, p.w_grad_f32 != 0);
       return launch<true, true, EPI_STORE>(a, bn, pairs, st);
