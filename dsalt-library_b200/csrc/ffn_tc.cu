@@ -523,7 +523,7 @@ cudaError_t launch_bn(const Args& a, int pairs, cudaStream_t st) {
 template <bool AMN, bool BMN, int EPI, int ACT = 0>
 cudaError_t launch(const Args& a, int bn, int pairs, cudaStream_t st) {
   if (bn == 256) return launch_bn<AMN, BMN, EPI, 256, ACT>(a, pairs, st);
-  if constexpr (AMN)
+  if constexpr (BMN && EPI == EPI_STORE)
     if (bn == 512) return launch_bn<AMN, BMN, EPI, 512, ACT>(a, pairs, st);
   if constexpr (!BMN)
     if (bn == 64) return launch_bn<AMN, BMN, EPI, 64, ACT>(a, pairs, st);
@@ -615,7 +615,7 @@ cudaError_t launch_ffn_tc(int stage, const DsaltGatedFfnParams& p, bool early, c
       a.n_seg = 2;
       const Job job = {p.T, p.d, p.dx, p.d};
       const Jobs jobs = {&job, 1};
-      const int bn = pick_bn(jobs, 2 * steps(a.K), false, true, pairs);
+      const int bn = pick_bn(jobs, 2 * steps(a.K), false, true, pairs, true);
       set_jobs(a, jobs, bn);
       set_out(a, false);
       if (!encode(&a.ma[0], dt, p.dg, p.T, p.F, p.ld_f, false, 128) || !encode(&a.ma[1], dt, p.du, p.T, p.F, p.ld_f, false, 128) ||
