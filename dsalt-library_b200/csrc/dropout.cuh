@@ -52,19 +52,21 @@ struct Dropout {
       m[2 * j + 1] = v[j] >= high ? 0xffffffffu : 0u;
     }
   }
-  // the masks of elements i … i + 7, any i
+  // the masks of elements i … i + 7, any i: of two blocks as bits, shifted into place
   __device__ __forceinline__ void masks8(uint64_t i, uint32_t* m) const {
     const uint32_t o = (uint32_t)i & 7u;
-    uint32_t a[16];
-    masks_block(i >> 3, a);
-    if (o) masks_block((i >> 3) + 1, a + 8);
+    uint32_t bits = 0;
+    masks_block(i >> 3, m);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      m[j] = a[j];
+    for (int j = 0; j < 8; ++j) bits |= m[j] & (1u << j);
+    if (o) {
+      masks_block((i >> 3) + 1, m);
 #pragma unroll
-      for (int k = 1; k < 8; ++k)
-        if (o == k) m[j] = a[j + k];
+      for (int j = 0; j < 8; ++j) bits |= m[j] & (256u << j);
     }
+    bits >>= o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m[j] = (uint32_t)((int32_t)(bits << (31 - j)) >> 31);
   }
 };
 
