@@ -28,7 +28,8 @@ def check_seed(seed, site: int, device: torch.device) -> None:
         raise TypeError("seed must be an int64 tensor of one element")
     if not 0 <= site < 2 ** 32:
         raise ValueError(f"site must be in [0, 2^32), got {site}")
-    _ext.same_device(device, seed=seed)
+    if seed.device != device:
+        _ext.same_device(device, seed=seed)
 
 
 def new_dropout_seed(device: torch.device) -> torch.Tensor:
@@ -40,8 +41,8 @@ def new_dropout_seed(device: torch.device) -> torch.Tensor:
 def _launch(x: torch.Tensor, seed: torch.Tensor, site: int, threshold: int) -> torch.Tensor:
     x = _ext.contiguous(x)
     y = torch.empty_like(x)
-    p = _ext.DropoutParams(x=x.data_ptr(), y=y.data_ptr(), seed=seed.data_ptr(), n=x.numel(), site=site,
-                           threshold=threshold, dtype=_ext.dtype_code(x.dtype))
+    p = _ext.DropoutParams(x.data_ptr(), y.data_ptr(), seed.data_ptr(), x.numel(), site, threshold,
+                           _ext.dtype_code(x.dtype))
     _ext.call_on(x.device, "dsalt_dropout", p)
     return y
 

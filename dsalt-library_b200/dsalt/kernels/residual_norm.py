@@ -94,9 +94,10 @@ class ResidualNormFunction(torch.autograd.Function):
         dx_new, dh = (None if t is None else _ext.contiguous(t) for t in (dx_new, dh))
         dx, df = torch.empty_like(f), torch.empty_like(f)
         dgate = None if gate is None else torch.empty_like(gate)
-        need = (ctx.needs_input_grad[2], ctx.needs_input_grad[3], ctx.needs_input_grad[5])
-        dpost, dscale, dnorm = (torch.empty_like(v) if v is not None and n else None
-                                for v, n in zip((post, scale, norm), need))
+        need = ctx.needs_input_grad
+        dpost = torch.empty_like(post) if post is not None and need[2] else None
+        dscale = torch.empty_like(scale) if scale is not None and need[3] else None
+        dnorm = torch.empty_like(norm) if norm is not None and need[5] else None
         parts = torch.empty(_parts(p.T, p.d, f.device.index), 2, p.d, dtype=torch.float32, device=f.device)
         p.rf, p.r, p.dx_new, p.dh = _ext.ptr(rf), _ext.ptr(r), _ext.ptr(dx_new), _ext.ptr(dh)
         p.dx, p.df, p.dgate, p.parts = dx.data_ptr(), df.data_ptr(), _ext.ptr(dgate), parts.data_ptr()
@@ -150,10 +151,14 @@ def residual_norm(x: torch.Tensor, f: torch.Tensor, norm_weight: torch.Tensor | 
         check_seed(seed, site, x.device)
     else:
         seed, site = None, 0
-    _ext.same_device(x.device, f=f, post_weight=post_weight, scale=scale, gate=gate, norm_weight=norm_weight)
-    x2, f2 = (t if t.dim() == 2 else t.reshape(-1, d) for t in (x, f))
-    leaves = (x, f, post_weight, scale, gate, norm_weight)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves):
+    dev = x.device
+    for t in (f, post_weight, scale, gate, norm_weight):
+        if t is not None and t.device != dev:
+            _ext.same_device(dev, f=f, post_weight=post_weight, scale=scale, gate=gate, norm_weight=norm_weight)
+    x2, f2 = (x, f) if x.dim() == 2 else (x.reshape(-1, d), f.reshape(-1, d))
+    grad = torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in
+                                            (x, f, post_weight, scale, gate, norm_weight)])
+    if grad:
         out = ResidualNormFunction.apply(x2, f2, post_weight, scale, gate, norm_weight, seed, float(eps), site,
                                          threshold, gate_mode)
         x_new, h = out if norm_weight is not None else (out, None)
