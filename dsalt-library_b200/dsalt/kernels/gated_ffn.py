@@ -51,21 +51,25 @@ def _params(x2, wg, wu, wd, activation: int, dtype: torch.dtype):
     return p
 
 
+def _set_kept(p, kept: torch.Tensor, keep: bool) -> None:
+    """The pointers into ``kept``: h, then with ``keep`` a, b and ab, then h's low words."""
+    step = 2 * p.T * p.ld_f
+    base = kept.data_ptr()
+    p.h, p.h_lo = base, base + (kept.shape[0] - 1) * step
+    if keep:
+        p.a, p.b, p.ab = base + step, base + 2 * step, base + 3 * step
+
+
 def _forward(x2, wg, wu, wd, activation: int, dtype: torch.dtype, keep: bool):
-    """``(y, h, a, b, ab)``; the last three, 16-bit words, only with ``keep``."""
+    """``(y, kept)``: ``kept`` holds what a backward needs (with ``keep``) and scratch, in 16-bit words."""
     p = _params(x2, wg, wu, wd, activation, dtype)
     T, dev = p.T, x2[0].device
-    # few tokens: h's rounding rests beside it (scratch)
-    h = torch.empty(2 * T if T <= _ext.FFN_FEW_TOKENS else T, p.ld_f, dtype=dtype, device=dev)
+    kept = torch.empty((4 if keep else 1) + (T <= _ext.FFN_FEW_TOKENS), T, p.ld_f, dtype=dtype, device=dev)
     y = torch.empty(T, p.d_out, dtype=dtype, device=dev)
-    p.h, p.y = h.data_ptr(), y.data_ptr()
-    p.h_lo = h.data_ptr() + 2 * T * p.ld_f
-    a = b = ab = None
-    if keep:
-        a, b, ab = (torch.empty(T, p.ld_f, dtype=dtype, device=dev) for _ in range(3))
-        p.a, p.b, p.ab = a.data_ptr(), b.data_ptr(), ab.data_ptr()
+    _set_kept(p, kept, keep)
+    p.y = y.data_ptr()
     _ext.call_on(dev, "dsalt_gated_ffn_fwd", p)
-    return y, h, a, b, ab
+    return y, kept
 
 
 class GatedFFNFunction(torch.autograd.Function):
@@ -73,40 +77,46 @@ class GatedFFNFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation: int, dtype: torch.dtype):
-        ops = [_operand(t, dtype) for t in (x, w_gate, w_up, w_down)]
-        y, *kept = _forward(*ops, activation, dtype, True)
-        ctx.save_for_backward(*(t for t, _ in ops), *kept)
-        ctx.strides = [ld for _, ld in ops]
+        (x_, ld_x), (wg, ld_wg), (wu, ld_wu), (wd, ld_wd) = ops = [_operand(t, dtype) for t in (x, w_gate, w_up, w_down)]
+        y, kept = _forward(*ops, activation, dtype, True)
+        ctx.save_for_backward(x_, wg, wu, wd, kept)
+        ctx.strides = (ld_x, ld_wg, ld_wu, ld_wd)
         ctx.activation, ctx.dtype = activation, dtype
-        ctx.dtypes = [t.dtype for t in (x, w_gate, w_up, w_down)]
+        ctx.dtypes = (x.dtype, w_gate.dtype, w_up.dtype, w_down.dtype)
         return y
 
     @staticmethod
     def backward(ctx, dy):
         _ext.first_derivative_only()
-        *ops, h, a, b, ab = ctx.saved_tensors
-        dtype, dev = ctx.dtype, h.device
+        *ops, kept = ctx.saved_tensors
+        dtype, dev = ctx.dtype, kept.device
         p = _params(*zip(ops, ctx.strides), ctx.activation, dtype)
+        _set_kept(p, kept, True)
         dy_, p.ld_dy = _operand(dy, dtype)
-        need_x, *need_w = ctx.needs_input_grad[:4]
-        p.h, p.a, p.b, p.ab, p.dy = h.data_ptr(), a.data_ptr(), b.data_ptr(), ab.data_ptr(), dy_.data_ptr()
-        if need_x or need_w[0] or need_w[1]:
-            dg, du = torch.empty_like(a), torch.empty_like(a)
-            p.dg, p.du = dg.data_ptr(), du.data_ptr()
-        grads = [None] * 4
+        p.dy = dy_.data_ptr()
+        need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
+        if need_x or need_g or need_u:
+            scratch = torch.empty(2, p.T, p.ld_f, dtype=dtype, device=dev)
+            p.dg = scratch.data_ptr()
+            p.du = p.dg and p.dg + 2 * p.T * p.ld_f
+        dx = dw_gate = dw_up = dw_down = None
         if need_x:
-            grads[0] = torch.empty(p.T, p.d, dtype=dtype, device=dev)
-            p.dx = grads[0].data_ptr()
-        if any(need_w):
-            # fp32 sums where a weight is not of the compute dtype: its gradient is rounded once
-            p.w_grad_f32 = int(any(dt != dtype for dt in ctx.dtypes[1:]))
-            out = torch.float32 if p.w_grad_f32 else dtype
-            shapes = ((p.F, p.d), (p.F, p.d), (p.d_out, p.F))
-            for i, (need, shape) in enumerate(zip(need_w, shapes)):
-                if need:
-                    grads[1 + i] = torch.empty(shape, dtype=out, device=dev)
-            p.dw_gate, p.dw_up, p.dw_down = (_ext.ptr(t) for t in grads[1:])
+            dx = torch.empty(p.T, p.d, dtype=dtype, device=dev)
+            p.dx = dx.data_ptr()
+        # fp32 sums where a weight is not of the compute dtype: its gradient is rounded once
+        p.w_grad_f32 = any(dt != dtype for dt in ctx.dtypes[1:])
+        out = torch.float32 if p.w_grad_f32 else dtype
+        if need_g:
+            dw_gate = torch.empty(p.F, p.d, dtype=out, device=dev)
+            p.dw_gate = dw_gate.data_ptr()
+        if need_u:
+            dw_up = torch.empty(p.F, p.d, dtype=out, device=dev)
+            p.dw_up = dw_up.data_ptr()
+        if need_d:
+            dw_down = torch.empty(p.d_out, p.F, dtype=out, device=dev)
+            p.dw_down = dw_down.data_ptr()
         _ext.call_on(dev, "dsalt_gated_ffn_bwd", p)
+        grads = (dx, dw_gate, dw_up, dw_down)
         return (*(t if t is None or t.dtype == dt else t.to(dt) for t, dt in zip(grads, ctx.dtypes)), None, None)
 
 
