@@ -99,7 +99,8 @@ def inputs(T, d, F, d_out, dtype, seed=0, grad=True):
 
 SIZES = [(16, 264, 72, 1000), (17, 1024, 200, 8), (31, 65, 130, 67), (33, 520, 1368, 520), (64, 72, 40, 136), (65, 200, 264, 136),
          (128, 264, 520, 264), (200, 129, 63, 258), (256, 512, 1408, 512), (384, 72, 136, 24), (385, 63, 129, 65),
-         (513, 200, 264, 136), (1, 8, 8, 8), (1, 64, 96, 64), (2, 1, 1, 1), (3, 17, 5, 9), (5, 40, 72, 40), (17, 72, 136, 24), (64, 256, 512, 256),
+         (513, 200, 264, 136), (20, 264, 520, 2504), (130, 1032, 136, 2504), (4, 1032, 2056, 40), (700, 2056, 264, 520),
+         (1, 8, 8, 8), (1, 64, 96, 64), (2, 1, 1, 1), (3, 17, 5, 9), (5, 40, 72, 40), (17, 72, 136, 24), (64, 256, 512, 256),
          (127, 64, 128, 64), (129, 200, 264, 136), (300, 96, 1000, 96), (257, 63, 129, 65), (640, 512, 1408, 512)]
 
 
