@@ -1,9 +1,9 @@
 // Between a block and the next one, in one pass each way:
-//   n  = f·rf·post (or f),  x' = R(x + D(scale⊙gate⊙n)),  h = R(x'·r·norm)
-// with rf and r the inverse root mean squares of f and x', D the dropout of
-// dropout.cuh and R the rounding to the tensors' type.  h is the norm of the
-// rounded x', the tensor that the next residual add and the backward see (as in
-// rmsnorm.cu's fused add).  Backward:
+//   n  = f·rf·post (or f),  s = x + D(scale⊙gate⊙n),  x' = R(s),  h = R(s·r·norm)
+// with rf and r the inverse root mean squares of f and s, D the dropout of
+// dropout.cuh and R the rounding to the tensors' type: h is the norm of the sum
+// before its rounding, so that it is off by one rounding and not by two.  Backward,
+// from the stored x':
 //   G = dx_new + r·(dh⊙norm − x'·r²·mean(dh⊙norm⊙x')),  dx = R(G),  dn = D(G)⊙scale⊙gate,
 //   df = R(rf·(dn⊙post − f·rf²·mean(dn⊙post⊙f))),  dgate = D(G)⊙scale⊙n,
 //   dscale = Σ_t D(G)⊙gate⊙n,  dpost = Σ_t dn⊙f·rf,  dnorm = Σ_t dh⊙x'·r.
@@ -212,7 +212,6 @@ __global__ void __launch_bounds__(MAXT, (CH == 1 ? 1024 : 512) / MAXT) residual_
       for (int j = 0; j < 4; ++j) x[ch][j] = fma2(f[ch][j], rf2, x[ch][j]);
       out.set(x[ch]);
       out.store(reinterpret_cast<T*>(p.x_new) + at, p.d - c);
-      out.get(x[ch]);  // the rounded x'
 #pragma unroll
       for (int j = 0; j < 4; ++j) s2 = fma2(x[ch][j], x[ch][j], s2);
     }

@@ -119,7 +119,7 @@ def residual_norm(x: torch.Tensor, f: torch.Tensor, norm_weight: torch.Tensor | 
     out: no norm of ``f``, no scale, no second norm (``h`` is then None).  ``gate``: x's
     dtype, one value per token (``[...]`` or ``[..., 1]``) or per element (``[..., d]``).
     Dropout draws as ``counter_dropout`` does for a tensor of x's shape.  ``h`` is the
-    norm of the rounded ``x_new``.  All sums are fp32.  First derivatives only; the
+    norm of the sum before it is rounded to ``x_new``.  All sums are fp32.  First derivatives only; the
     gradients of the vectors are summed in a fixed order.
     """
     _ext.require_cuda(x, "x")

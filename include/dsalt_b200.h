@@ -557,8 +557,8 @@ DSALT_API int dsalt_dropout(const DsaltDropoutParams* p, void* stream);
 /* Between a block and the next: the norm of the block's output f, its gate and
  * residual scale, dropout, the residual add and the norm before the next block.
  *   n  = f·rf·post,  rf = 1/sqrt(mean(f²) + eps)         (n = f without post)
- *   x' = R(x + D(scale⊙gate⊙n)),  D as dsalt_dropout on [T, d]
- *   h  = R(x'·r·norm), r = 1/sqrt(mean(x'²) + eps)       (with norm set)
+ *   s  = x + D(scale⊙gate⊙n), x' = R(s),  D as dsalt_dropout on [T, d]
+ *   h  = R(s·r·norm), r = 1/sqrt(mean(s²) + eps)         (with norm set)
  * and the backward, from the gradients of x' (dx_new) and h (dh), either NULL for 0:
  *   G  = dx_new + r·(dh⊙norm − x'·r²·mean(dh⊙norm⊙x')),  dx = R(G),
  *   dn = D(G)⊙scale⊙gate,  df = R(rf·(dn⊙post − f·rf²·mean(dn⊙post⊙f))),

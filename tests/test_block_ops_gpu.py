@@ -72,8 +72,8 @@ def test_operator_chain_against_64_bits():
         return t / torch.sqrt((t * t).mean(-1, keepdim=True) + 1e-6) * w
 
     D = lambda t: t.double()  # noqa: E731
-    for got, ref in ((x1, D(x) + D(sc) * D(a)), (h, norm(D(x1), D(w1))), (x2, D(x1) + norm(D(f), D(w1))),
-                     (h2, norm(D(x2), D(w2)))):
+    s1, s2 = D(x) + D(sc) * D(a), D(x1) + norm(D(f), D(w1))
+    for got, ref in ((x1, s1), (h, norm(s1, D(w1))), (x2, s2), (h2, norm(s2, D(w2)))):
         assert ((D(got) - ref).abs() <= 2 * e * ref.abs() + 2.0 ** -16).all()
     hid = F.silu(D(h) @ D(wg).t()) * (D(h) @ D(wu).t())
     ref = hid @ D(wd).t()

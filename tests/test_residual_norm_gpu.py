@@ -1,7 +1,7 @@
 """GPU tests of the fused residual step against its formulas in 64 bits.
 
 The 64-bit formulas take the kernel's own rounded ``x_new`` where the definition does
-(``h`` and the backward).  Bounds: each result is rounded once to its type (e of the
+(the backward; ``h`` is the norm of the sum before its rounding).  Bounds: each result is rounded once to its type (e of the
 value) from fp32 sums and products; those are off by c = 2^-18 of the sum of the
 terms' magnitudes (row sums of up to 2^6·8 terms a thread and a tree, a reciprocal
 square root of 2 ulp, fewer than 20 products).  Sums over T rows: T·2^-24 more.
@@ -54,12 +54,12 @@ def reference(t, x_new, dx_new, dh, mask, eps=1e-6):
     n = f * rf * post
     branch = mask * scale * gate * n
     out = {"x_new": (v["x"] + branch, v["x"].abs() + branch.abs())}
-    xn = x_new.detach().double()
-    r = 1 / torch.sqrt((xn * xn).mean(-1, keepdim=True) + eps)
+    xn, s = x_new.detach().double(), out["x_new"][0]
+    r = 1 / torch.sqrt((s * s).mean(-1, keepdim=True) + eps)
     G = torch.zeros_like(xn) if dx_new is None else dx_new.double()
     mag = G.abs()
     if v["norm"] is not None:
-        out["h"] = (xn * r * v["norm"], (xn * r * v["norm"]).abs())
+        out["h"] = (s * r * v["norm"], (out["x_new"][1] + s.abs()) * r * v["norm"].abs())
         if dh is not None:
             q = dh.double() * v["norm"]
             G = G + r * (q - xn * r * r * (q * xn).mean(-1, keepdim=True))
@@ -167,7 +167,7 @@ def test_same_draws_as_counter_dropout_and_same_sum_as_add_rms_norm():
     xb, fb = x.bfloat16(), f.bfloat16()
     got, ref = residual_norm(xb, fb, w, eps=1e-6), add_rms_norm(xb, fb, w, 1e-6)
     assert torch.equal(got[0], ref[0])
-    # two roundings of values that differ by fp32 rounding: one step of the type
+    # the norm of the sum before and after its rounding, each rounded: 3 · 2^-9
     assert ((got[1].float() - ref[1].float()).abs() <= 2.0 ** -7 * ref[1].float().abs()).all()
 
 
