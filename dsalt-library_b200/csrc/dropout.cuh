@@ -36,6 +36,18 @@ struct Dropout {
     const uint64_t s = threshold_ > 0 ? (uint64_t)__ldg(seed) : 0;
     key = make_uint2((uint32_t)s, (uint32_t)(s >> 32));
   }
+  // v, 8·block … 8·block + 7, with 0 where dropped
+  __device__ __forceinline__ void select_block(uint64_t block, float* v) const {
+    const uint4 w = philox(make_uint4((uint32_t)block, (uint32_t)(block >> 32), site, 0u), key);
+    const uint32_t d[4] = {w.x, w.y, w.z, w.w};
+    const uint32_t high = threshold << 16;
+    const bool some = threshold < 65536;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = some && (d[j] << 16) >= high ? v[2 * j] : 0.f;
+      v[2 * j + 1] = some && d[j] >= high ? v[2 * j + 1] : 0.f;
+    }
+  }
   // m[j] = all ones where element 8·block + j is kept, 0 where it is dropped
   __device__ __forceinline__ void masks_block(uint64_t block, uint32_t* m) const {
     const uint4 w = philox(make_uint4((uint32_t)block, (uint32_t)(block >> 32), site, 0u), key);

@@ -9,8 +9,8 @@
 //   dscale = Σ_t D(G)⊙gate⊙n,  dpost = Σ_t dn⊙f·rf,  dnorm = Σ_t dh⊙x'·r.
 // Everything between the loads and the stores is fp32.  Bound by the rows' bytes, once in
 // and once out, and with dropout by issue slots (the generator's ten rounds a block of
-// eight elements).  16384 × 1024 bf16 with every part: forward 43 us (30 without dropout;
-// 134 MB), backward 61 us (49; 201 MB).
+// eight elements).  16384 × 1024 bf16 with every part: forward 41 us (29 without dropout;
+// 134 MB), backward 61 us (48; 201 MB).
 //
 // A row belongs to a group of threads of eight consecutive columns each: 8, 16 or
 // 32 lanes of a warp up to d = 256, else a whole CTA (of one, two or four chunks of
@@ -40,7 +40,7 @@ struct Shape {
 };
 // Two chunks a thread past d = 4096, and from d = 512 on where rows are read element by
 // element (16384 × 1001 bf16: 229 us instead of 276 with one); one elsewhere (16384 × 1024:
-// 109 us instead of 117 with two).
+// 109 us instead of 117 with two, before the forward selected instead of masking).
 inline Shape shape_of(int d, bool vec) {
   const int units = (d + 7) / 8;
   if (units <= 8) return {8, kSmallThreads, 1};
@@ -195,17 +195,28 @@ __global__ void __launch_bounds__(MAXT, (CH == 1 ? 1024 : 512) / MAXT) residual_
       const int64_t at = row + c;
       f2 (&wb)[4] = wbs[ch], (&wn)[4] = wns[ch];
       if (!kHold) column_factors<T>(p, dr, c, wb, wn);
-      uint32_t m[8];
-      row_masks<VEC, DROP>(dr, at, m);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) f[ch][j] = mul2(and2(f[ch][j], m[2 * j], m[2 * j + 1]), wb[j]);
+      for (int j = 0; j < 4; ++j) f[ch][j] = mul2(f[ch][j], wb[j]);
       if (p.gate_mode == DSALT_GATE_FULL) {
         Raw<T, VEC> raw;
         f2 g[4];
         raw.load(Gt + at, p.d - c);
         raw.get(g);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[ch][j] = mul2(f[ch][j], and2(g[j], m[2 * j], m[2 * j + 1]));
+        for (int j = 0; j < 4; ++j) f[ch][j] = mul2(f[ch][j], g[j]);
+      }
+      if constexpr (DROP && VEC) {
+        float e[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) unpair(f[ch][j], e[2 * j], e[2 * j + 1]);
+        dr.select_block((uint64_t)at >> 3, e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[ch][j] = pair(e[2 * j], e[2 * j + 1]);
+      } else if constexpr (DROP) {
+        uint32_t m[8];
+        dr.masks8((uint64_t)at, m);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[ch][j] = and2(f[ch][j], m[2 * j], m[2 * j + 1]);
       }
       Raw<T, VEC> out;
 #pragma unroll
