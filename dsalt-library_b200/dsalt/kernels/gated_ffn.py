@@ -35,9 +35,7 @@ def _operand(t: torch.Tensor, dtype: torch.dtype):
         if rows == 1:
             return t, (cols + 7) // 8 * 8
     ld = (cols + 7) // 8 * 8
-    buf = torch.empty(rows, ld, dtype=dtype, device=t.device)
-    buf[:, :cols].copy_(t)
-    return buf[:, :cols], ld
+    return torch.empty_strided((rows, cols), (ld, 1), dtype=dtype, device=t.device).copy_(t), ld
 
 
 def _params(x2, wg, wu, wd, activation: int, dtype: torch.dtype):
