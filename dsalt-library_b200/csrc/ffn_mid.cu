@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(kThreads) ffn_mid_kernel(const __grid_constant
   // -------------------------------------------------------- partial sums
   // (also after a wait that gave up: the cluster's barriers are met by all its CTAs)
   const bool ok = mbar_wait(bar[C::ACC], 0, abort_flag, p.status);
+  __syncwarp();  // the lanes' waits may end apart; the TMEM loads want them together
   tc_fence_after();
   __syncthreads();  // every product and copy of this CTA is done: the ring becomes the sums
   float* sums = reinterpret_cast<float*>(sm.ring);
@@ -216,6 +217,7 @@ __global__ void __launch_bounds__(kThreads) ffn_mid_kernel(const __grid_constant
       put(p.out_lo, pack2(v[0] - f0.x, v[1] - f0.y, p.bf16), pack2(v[2] - f1.x, v[3] - f1.y, p.bf16));
     }
   }
+  __syncwarp();  // the loop above ends lane by lane; the barriers and the release of TMEM want whole warps
   if (p.split > 1) cluster_sync();  // no CTA leaves while its sums are read
   else __syncthreads();
   tc_fence_after();
