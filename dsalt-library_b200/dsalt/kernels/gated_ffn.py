@@ -75,10 +75,9 @@ class GatedFFNFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation: int, dtype: torch.dtype):
-        (x_, ld_x), (wg, ld_wg), (wu, ld_wu), (wd, ld_wd) = ops = [_operand(t, dtype) for t in (x, w_gate, w_up, w_down)]
+        ops = [_operand(t, dtype) for t in (x, w_gate, w_up, w_down)]
         y, kept = _forward(*ops, activation, dtype, True)
-        ctx.save_for_backward(x_, wg, wu, wd, kept)
-        ctx.strides = (ld_x, ld_wg, ld_wu, ld_wd)
+        ctx.save_for_backward(*(t for t, _ in ops), kept)
         ctx.activation, ctx.dtype = activation, dtype
         ctx.dtypes = (x.dtype, w_gate.dtype, w_up.dtype, w_down.dtype)
         return y
@@ -88,7 +87,9 @@ class GatedFFNFunction(torch.autograd.Function):
         _ext.first_derivative_only()
         *ops, kept = ctx.saved_tensors
         dtype, dev = ctx.dtype, kept.device
-        p = _params(*zip(ops, ctx.strides), ctx.activation, dtype)
+        # a saved tensor's layout is what came back: hooks (save_on_cpu) return dense copies
+        ops = [_operand(t, dtype) for t in ops]
+        p = _params(*ops, ctx.activation, dtype)
         _set_kept(p, kept, True)
         dy_, p.ld_dy = _operand(dy, dtype)
         p.dy = dy_.data_ptr()

@@ -27,3 +27,38 @@ def test_results_of_part_of_a_warp(size):
         check(g, ref[name], name)
     with torch.no_grad():
         assert all(torch.equal(gated_ffn(*leaves), y) for _ in range(10))
+
+
+@pytest.mark.parametrize("size", [(37, 64, 96, 40), (140, 710, 769, 710), (1, 17, 5, 9)])
+def test_gradients_of_operands_saved_on_the_host(size):
+    """torch's save_on_cpu brings slices and padded copies back as dense tensors: the same bits."""
+    from dsalt.kernels.gated_ffn import gated_ffn
+    T, d, F, _ = size
+    x, wg, wu, wd, dy = inputs(*size, torch.bfloat16, grad=False)
+    pad = (-d) % 8 + 16
+    xs = torch.nn.functional.pad(x, (0, pad))[:, :d].requires_grad_(True)
+    stacked = torch.nn.functional.pad(torch.stack([wg, wu]), (0, pad))
+    leaves = [xs, *(w[:, :d].requires_grad_(True) for w in stacked), wd.requires_grad_(True)]
+    ref = torch.autograd.grad(gated_ffn(*leaves), leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = gated_ffn(*leaves)
+    got = torch.autograd.grad(y, leaves, dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+def test_residual_step_and_dropout_saved_on_the_host():
+    from dsalt import counter_dropout, residual_norm
+    seed = torch.tensor([3], dtype=torch.int64, device="cuda")
+    x, f = (torch.randn(60, 264, device="cuda").bfloat16().requires_grad_(True) for _ in range(2))
+    w = torch.rand(264, device="cuda").requires_grad_(True)
+    gate = torch.rand(60, 528, device="cuda").bfloat16()[:, ::2].requires_grad_(True)
+    leaves = (x, f, w, gate)
+
+    def step():
+        x_new, h = residual_norm(x, counter_dropout(f, 0.25, seed, 1), w, post_weight=w, gate=gate, dropout_p=0.25, seed=seed)
+        return x_new.float().sum() + h.float().square().sum()
+
+    ref = torch.autograd.grad(step(), leaves)
+    with torch.autograd.graph.save_on_cpu():
+        y = step()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves), ref))
