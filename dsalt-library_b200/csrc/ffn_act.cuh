@@ -2,6 +2,8 @@
 // forward keeps of them, shared by the kernels for many and for few tokens.
 #pragma once
 
+#include <math_constants.h>
+
 #include "tc_pair.cuh"
 
 namespace dsalt {
@@ -57,6 +59,11 @@ __device__ __forceinline__ void act_pair(float g, float& a, float& da) {
 __device__ __forceinline__ float2 unpack2(uint32_t w, bool bf16) {
   if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+// What v's rounding to the 16-bit value `high` leaves.  0 beside an infinity or NaN, which
+// v − high would meet with an infinity of the other sign.
+__device__ __forceinline__ float rounding_rest(float v, float high) {
+  return fabsf(high) < CUDART_INF_F ? v - high : 0.f;
 }
 // Upper 16 bits of fp32 x (low half) and y: the words of a and b.
 __device__ __forceinline__ uint32_t upper16(float x, float y) {

@@ -184,7 +184,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) ffn_few_kernel(const FewArgs p
     const uint32_t word = sm100::pack2(result, result, BF16);
     p.out[at] = (uint16_t)(word & 0xffffu);
     if constexpr (NM == 2) {
-      const float rest = result - (BF16 ? __uint_as_float(word << 16) : __half2float(__ushort_as_half((uint16_t)word)));
+      const float rest =
+          rounding_rest(result, BF16 ? __uint_as_float(word << 16) : __half2float(__ushort_as_half((uint16_t)word)));
       p.h_lo[at] = (uint16_t)(sm100::pack2(rest, rest, BF16) & 0xffffu);
     }
   }

@@ -214,7 +214,8 @@ __global__ void __launch_bounds__(kThreads) ffn_mid_kernel(const __grid_constant
     put(p.out, w0, w1);
     if (HIDDEN && p.out_lo) {
       const float2 f0 = unpack2(w0, p.bf16), f1 = unpack2(w1, p.bf16);
-      put(p.out_lo, pack2(v[0] - f0.x, v[1] - f0.y, p.bf16), pack2(v[2] - f1.x, v[3] - f1.y, p.bf16));
+      put(p.out_lo, pack2(rounding_rest(v[0], f0.x), rounding_rest(v[1], f0.y), p.bf16),
+          pack2(rounding_rest(v[2], f1.x), rounding_rest(v[3], f1.y), p.bf16));
     }
   }
   __syncwarp();  // the loop above ends lane by lane; the barriers and the release of TMEM want whole warps

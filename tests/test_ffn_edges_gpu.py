@@ -62,3 +62,36 @@ def test_residual_step_and_dropout_saved_on_the_host():
     with torch.autograd.graph.save_on_cpu():
         y = step()
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves), ref))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T", [1, 4, 16, 24, 40, 64, 70, 400])
+def test_hidden_values_past_the_type(T, dtype):
+    """A hidden value that the type holds only as an infinity makes the outputs that use it
+    infinite, or NaN where infinities of both signs or a weight of 0 meet, at any number of
+    tokens: only the sum's infinities, none that the split into two words brings in."""
+    from dsalt.kernels.gated_ffn import gated_ffn
+    d, F, d_out = 32, 48, 24
+    x, wg, wu, wd, _ = inputs(T, d, F, d_out, dtype, grad=False)
+    big = 300.0 if dtype == torch.float16 else 2.0 ** 65  # its square is past the type
+    x[:, 0] = 0
+    x[::2, 0] = 1.0                                # every other token
+    wg[:, 0], wu[:, 0] = 0, 0
+    wg[5, 0] = wu[5, 0] = wg[20, 0] = big          # h[5] past the type, h[20] not
+    wg[5, 1:], wu[5, 1:], wg[20, 1:] = 0, 0, 0
+    wd[:4, 5], wd[4:8, 5], wd[8:12, 5] = 0.5, -0.5, 0
+    wg[30, 0], wu[30, 0], wg[30, 1:], wu[30, 1:] = big, -big, 0, 0   # h[30] past it with the other sign
+    wd[:, 30] = 0.0
+    wd[12:, 30], wd[12:, 5] = 0.25, 0.25           # inf - inf
+    y = gated_ffn(x, wg, wu, wd)
+    on, off = y[::2], y[1::2]
+    assert torch.isfinite(off).all()
+    # weights of 0 times an infinity are NaN: columns 0 to 11 have h[30] · 0
+    assert torch.isnan(on).all()
+    wd[:, 30] = 1e-3
+    wu[30] = 0                                     # h[30] = 0: one infinity alone
+    y = gated_ffn(x, wg, wu, wd)
+    on = y[::2]
+    assert (on[:, :4] == float("inf")).all() and (on[:, 4:8] == -float("inf")).all()
+    assert torch.isnan(on[:, 8:12]).all() and (on[:, 12:] == float("inf")).all()
+    assert torch.isfinite(y[1::2]).all()
