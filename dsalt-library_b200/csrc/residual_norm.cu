@@ -18,12 +18,15 @@
 // on their way, its weights and column sums in registers; the sums of a CTA go to one
 // partial row and a second kernel adds the partial rows in order.
 //
-// The backward needs Σ dh⊙norm⊙x' before G, and Σ κ⊙G with κ = D⊙scale⊙post⊙f, times a
-// full gate (for df and a token's dgate), after it.  G = u − e·x' with
-// u = dx_new + r·dh⊙norm and e = r³·mean(dh⊙norm⊙x') is linear in that first sum, so
-// Σ κ⊙G = Σ κ⊙u − e·Σ κ⊙x': one round of three sums a row instead of two dependent rounds.
-// dscale and dpost share one sum over the rows, A = Σ_t D(G)⊙gate⊙f·rf: dscale = post⊙A,
-// dpost = scale⊙A.
+// The backward works on the normed rows x̂ = x'·r and f̂ = f·rf, which stay near 1 whatever
+// the rows' size: the cube of an inverse root mean square would leave fp32's range at rows
+// of 1e13 (and, with a small eps, of 1e-13).  With q = dh⊙norm,
+//   G = dx_new + r·(q − x̂·mean(q⊙x̂)),  df = rf·(dn⊙post − f̂·mean(dn⊙post⊙f̂)).
+// It needs Σ q⊙x̂ before G, and Σ κ⊙G with κ = D⊙scale⊙post⊙f̂, times a full gate (for df
+// and a token's dgate), after it.  G = u − e·x̂ with u = dx_new + r·q and e = r·mean(q⊙x̂)
+// is linear in that first sum, so Σ κ⊙G = Σ κ⊙u − e·Σ κ⊙x̂: one round of three sums a row
+// instead of two dependent rounds.  dscale and dpost share one sum over the rows,
+// A = Σ_t D(G)⊙gate⊙f̂: dscale = post⊙A, dpost = scale⊙A.
 #include <algorithm>
 
 #include "dropout.cuh"
@@ -303,8 +306,8 @@ __global__ void __launch_bounds__(MAXT, CH == 1 ? 512 / MAXT : 1) residual_bwd_k
   for (int k = 0; k < rounds; ++k, t += stride, row += stride * p.d) {
     const bool on = t < p.T;
     const float r = nr, rf = nrf, gt = ngt;
-    const f2 r2 = dup(r);
-    f2 u[CH][4], x[CH][4], f[CH][4];
+    const f2 r2 = dup(r), rf2 = dup(rf);
+    f2 u[CH][4], x[CH][4], f[CH][4];  // x̂, f̂
     uint32_t m[CH][8];
     f2 s0 = dup(0.f), s1 = dup(0.f), s2 = dup(0.f);
 #pragma unroll
@@ -326,10 +329,12 @@ __global__ void __launch_bounds__(MAXT, CH == 1 ? 512 / MAXT : 1) residual_bwd_k
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
+        x[ch][j] = mul2(x[ch][j], r2);
         const f2 hx = mul2(dh[j], x[ch][j]);
-        a_norm[ch][j] = fma2(hx, r2, a_norm[ch][j]);
+        a_norm[ch][j] = add2(hx, a_norm[ch][j]);
         s0 = fma2(hx, wn[j], s0);
         u[ch][j] = fma2(mul2(dh[j], wn[j]), r2, u[ch][j]);
+        if (POST) f[ch][j] = mul2(f[ch][j], rf2);
         // κ: a dropped element passes nothing back, whatever f holds there
         f2 kf = and2(f[ch][j], m[ch][2 * j], m[ch][2 * j + 1]);
         if (!POST) f[ch][j] = kf;
@@ -342,10 +347,10 @@ __global__ void __launch_bounds__(MAXT, CH == 1 ? 512 / MAXT : 1) residual_bwd_k
     if (kHold && k + 1 < rounds) fetch(t + stride, row + stride * p.d);
     float s[3] = {sum8(s0), sum8(s1), sum8(s2)};
     if (sums) group_sum(s, group, red[k & 1]);
-    const float e = r * r * r * (s[0] * inv_d);
+    const float e = r * (s[0] * inv_d);
     const float S = fmaf(-e, s[2], s[1]);  // Σ κ⊙G, without a token's gate
-    if (p.gate_mode == DSALT_GATE_TOKEN && on && lane == 0) reinterpret_cast<T*>(p.dgate)[t] = from_f32<T>(rf * S);
-    const f2 ne = dup(-e), al = dup(rf * gt), nm = dup(-rf * rf * rf * gt * (S * inv_d));
+    if (p.gate_mode == DSALT_GATE_TOKEN && on && lane == 0) reinterpret_cast<T*>(p.dgate)[t] = from_f32<T>(S);
+    const f2 ne = dup(-e), gt2 = dup(gt), al = dup(rf * gt), nm = dup(-(rf * gt) * (S * inv_d));
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (lane + ch * group) * 8;
@@ -367,9 +372,9 @@ __global__ void __launch_bounds__(MAXT, CH == 1 ? 512 / MAXT : 1) residual_bwd_k
         for (int j = 0; j < 4; ++j) {
           const f2 G = and2(u[ch][j], m[ch][2 * j], m[ch][2 * j + 1]);
           const f2 Gw = mul2(G, wb[j]);
-          dg[j] = mul2(mul2(Gw, f[ch][j]), al);
+          dg[j] = mul2(Gw, f[ch][j]);
           df[j] = mul2(mul2(Gw, g[j]), al);
-          a_branch[ch][j] = fma2(mul2(mul2(G, g[j]), f[ch][j]), al, a_branch[ch][j]);
+          a_branch[ch][j] = fma2(mul2(G, g[j]), f[ch][j], a_branch[ch][j]);
         }
         out.set(dg);
         out.store(reinterpret_cast<T*>(p.dgate) + at, p.d - c);
@@ -378,7 +383,7 @@ __global__ void __launch_bounds__(MAXT, CH == 1 ? 512 / MAXT : 1) residual_bwd_k
         for (int j = 0; j < 4; ++j) {
           const f2 G = and2(u[ch][j], m[ch][2 * j], m[ch][2 * j + 1]);
           df[j] = mul2(mul2(G, wb[j]), al);
-          a_branch[ch][j] = fma2(mul2(G, f[ch][j]), al, a_branch[ch][j]);
+          a_branch[ch][j] = fma2(mul2(G, f[ch][j]), gt2, a_branch[ch][j]);
         }
       }
       if (POST) {
@@ -390,8 +395,8 @@ __global__ void __launch_bounds__(MAXT, CH == 1 ? 512 / MAXT : 1) residual_bwd_k
     }
     if (!kHold && k + 1 < rounds) fetch(t + stride, row + stride * p.d);
   }
-  // this CTA's sums: partial row blockIdx.x of [CTAs][2][d] (Σ G⊙gate⊙f·rf where kept,
-  // Σ dh⊙x'·r); several groups' sums are added in order first
+  // this CTA's sums: partial row blockIdx.x of [CTAs][2][d] (Σ G⊙gate⊙f̂ where kept,
+  // Σ dh⊙x̂); several groups' sums are added in order first
   float* part = p.parts + (int64_t)blockIdx.x * 2 * p.d;
   if (per_cta > 1) {
     __shared__ float group_sums[CH == 1 && MAXT == 256 ? 2 * kSmallThreads * 8 : 1];
