@@ -12,6 +12,7 @@ import os
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB_PATH = Path(__file__).resolve().parents[1] / "_lib" / "libdsalt_b200.so"
 
@@ -284,6 +285,15 @@ def call_on(device: torch.device, name: str, params) -> None:
 
 def contiguous(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
+
+
+def differentiates(*tensors) -> bool:
+    """Whether a call has to go through its autograd Function: one of ``tensors`` (None is
+    skipped) requires a gradient, or forward mode is on, whose tangents ``requires_grad``
+    does not show and a Function without a rule for them refuses."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors])
 
 
 def first_derivative_only() -> None:

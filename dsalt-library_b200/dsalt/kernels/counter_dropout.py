@@ -70,7 +70,8 @@ def counter_dropout(x: torch.Tensor, p: float, seed: torch.Tensor, site: int = 0
     Kept elements are divided by the share kept; dropped ones are 0 whatever ``x``
     holds there.  ``x`` itself comes back when nothing is dropped (``p`` rounds to 0, or
     not ``training``).  ``seed`` (int64, one element, on x's device) must not be
-    changed before the backward has run: autograd then raises.
+    changed before the backward has run: autograd then raises.  First derivatives in
+    reverse mode only.
     """
     threshold = drop_threshold(p)
     _ext.require_cuda(x, "x")
@@ -78,6 +79,6 @@ def counter_dropout(x: torch.Tensor, p: float, seed: torch.Tensor, site: int = 0
     if not training or threshold == 0:
         return x
     check_seed(seed, site, x.device)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _ext.differentiates(x):
         return CounterDropoutFunction.apply(x, seed, site, threshold)
     return _launch(x, seed, site, threshold)

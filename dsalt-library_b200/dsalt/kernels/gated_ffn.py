@@ -143,7 +143,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     compute dtype; by default autocast's, or the one 16-bit dtype of all four tensors.
     Tensors of other dtypes are cast to it and get gradients of their own dtype.
     Operands are read in place when their rows are contiguous and 16-byte aligned
-    (a slice of a stacked weight is), else copied first.  First derivatives only.
+    (a slice of a stacked weight is), else copied first.  First derivatives in reverse mode only.
     """
     _check(x, w_gate, w_up, w_down, activation)
     if dtype is None:
@@ -154,8 +154,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     flat = x.dim() == 2
     x2 = x if flat else x.reshape(-1, x.shape[-1])
     act = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
-                                    or w_down.requires_grad):
+    if _ext.differentiates(x, w_gate, w_up, w_down):
         y = GatedFFNFunction.apply(x2, w_gate, w_up, w_down, act, dtype)
     else:
         y = _forward(_operand(x2, dtype), _operand(w_gate, dtype), _operand(w_up, dtype), _operand(w_down, dtype), act,

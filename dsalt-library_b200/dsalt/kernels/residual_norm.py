@@ -119,8 +119,8 @@ def residual_norm(x: torch.Tensor, f: torch.Tensor, norm_weight: torch.Tensor | 
     out: no norm of ``f``, no scale, no second norm (``h`` is then None).  ``gate``: x's
     dtype, one value per token (``[...]`` or ``[..., 1]``) or per element (``[..., d]``).
     Dropout draws as ``counter_dropout`` does for a tensor of x's shape.  ``h`` is the
-    norm of the sum before it is rounded to ``x_new``.  All sums are fp32.  First derivatives only; the
-    gradients of the vectors are summed in a fixed order.
+    norm of the sum before it is rounded to ``x_new``.  All sums are fp32.  First derivatives in
+    reverse mode only; the gradients of the vectors are summed in a fixed order.
     """
     _ext.require_cuda(x, "x")
     _ext.dtype_code(x.dtype)
@@ -156,9 +156,7 @@ def residual_norm(x: torch.Tensor, f: torch.Tensor, norm_weight: torch.Tensor | 
         if t is not None and t.device != dev:
             _ext.same_device(dev, f=f, post_weight=post_weight, scale=scale, gate=gate, norm_weight=norm_weight)
     x2, f2 = (x, f) if x.dim() == 2 else (x.reshape(-1, d), f.reshape(-1, d))
-    grad = torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in
-                                            (x, f, post_weight, scale, gate, norm_weight)])
-    if grad:
+    if _ext.differentiates(x, f, post_weight, scale, gate, norm_weight):
         out = ResidualNormFunction.apply(x2, f2, post_weight, scale, gate, norm_weight, seed, float(eps), site,
                                          threshold, gate_mode)
         x_new, h = out if norm_weight is not None else (out, None)

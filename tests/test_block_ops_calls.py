@@ -52,3 +52,33 @@ def test_saved_operands_may_come_back_in_another_layout(launches, sizes):
         assert ld % 8 == 0
         if ptr in back and rows > 1:
             assert ld == back[ptr].stride(0)
+
+
+def dual_calls():
+    from dsalt import counter_dropout, gated_ffn, residual_norm
+    half, seed = torch.bfloat16, torch.tensor([1])
+    x, w, v, d = (torch.randn(*s).to(half) for s in ((4, 8), (16, 8), (8, 16), (8,)))
+    gate = torch.rand(4).to(half)
+    return {"gated_ffn": (lambda *t: gated_ffn(*t, dtype=half), (x, w, w.clone(), v)),
+            "residual_norm": (lambda a, f, n, p, s, g: residual_norm(a, f, n, post_weight=p, scale=s, gate=g)[0],
+                              (x, x.clone(), d, d.clone(), d.clone(), gate)),
+            "counter_dropout": (lambda t: counter_dropout(t, 0.5, seed), (x,))}
+
+
+@pytest.mark.parametrize("no_grad", [False, True])
+@pytest.mark.parametrize("name", ["gated_ffn", "residual_norm", "counter_dropout"])
+def test_forward_mode_is_refused(launches, name, no_grad):
+    """A tangent on any input raises: without a rule for it the result would silently carry
+    none, a derivative of 0."""
+    import torch.autograd.forward_ad as fw
+    fn, args = dual_calls()[name]
+    with torch.set_grad_enabled(not no_grad):
+        for i in range(len(args)):
+            with fw.dual_level():
+                dual = [fw.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(args)]
+                with pytest.raises(NotImplementedError, match="jvp"):
+                    fn(*dual)
+                assert fw.unpack_dual(torch.as_tensor(fn(*args))).tangent is None  # no tangent: no refusal
+        del launches[:]
+        fn(*args)
+        assert len(launches) == 1
