@@ -17,6 +17,7 @@
 // its first weights before it waits for h.
 #include <algorithm>
 
+#include "device.cuh"
 #include "ffn.cuh"
 #include "ffn_act.cuh"
 
@@ -190,20 +191,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) ffn_few_kernel(const FewArgs p
     }
   }
   if (p.split > 1) sm100::cluster_sync();  // no CTA leaves while its sums are read
-}
-
-cudaError_t sm_count(int* out) {
-  static int counts[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (counts[dev] <= 0) {
-    e = cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return e;
-  }
-  *out = counts[dev];
-  return cudaSuccess;
 }
 
 template <int NT, int NM, bool BF16, int ACT>

@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <cstring>
 
+#include "device.cuh"
 #include "ffn.cuh"
 #include "ffn_act.cuh"
 
@@ -223,20 +224,6 @@ __global__ void __launch_bounds__(kThreads) ffn_mid_kernel(const __grid_constant
   else __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, NT);
-}
-
-cudaError_t sm_count(int* out) {
-  static int counts[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (counts[dev] <= 0) {
-    e = cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return e;
-  }
-  *out = counts[dev];
-  return cudaSuccess;
 }
 
 bool encode(CUtensorMap* m, int dtype, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows) {

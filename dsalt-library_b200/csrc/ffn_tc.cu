@@ -42,6 +42,7 @@
 #include <cstring>
 #include <initializer_list>
 
+#include "device.cuh"
 #include "ffn.cuh"
 #include "ffn_act.cuh"
 
@@ -438,20 +439,6 @@ bool encode(CUtensorMap* m, int dtype, const void* base, int64_t rows, int64_t c
   return encode_tensor_map_3d(m, map_type(dtype), base, (uint64_t)cols, (uint64_t)rows, 1, (uint64_t)ld * 2, (uint64_t)ld * 2,
                               64, mn ? 64 : w, 1) == CUDA_SUCCESS;
 }
-cudaError_t sm_count(int* out) {
-  static int counts[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (counts[dev] <= 0) {
-    e = cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return e;
-  }
-  *out = counts[dev];
-  return cudaSuccess;
-}
-
 // The products of one launch, before the tile width is chosen.
 struct Job { int64_t M, N; void* out; int64_t ld_out; };
 struct Jobs {

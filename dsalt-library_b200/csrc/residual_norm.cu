@@ -29,6 +29,7 @@
 // A = Σ_t D(G)⊙gate⊙f̂: dscale = post⊙A, dpost = scale⊙A.
 #include <algorithm>
 
+#include "device.cuh"
 #include "dropout.cuh"
 
 namespace dsalt {
@@ -464,20 +465,6 @@ __global__ void __launch_bounds__(1024) residual_colsum_kernel(const DsaltResidu
   v *= p.threshold >= 65536 ? 0.f : 65536.f / (float)(65536 - p.threshold);
   put(p.dscale, v * weight(p.post));
   put(p.dpost, v * weight(p.scale));
-}
-
-cudaError_t sm_count(int* out) {
-  static int counts[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (counts[dev] <= 0) {
-    e = cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return e;
-  }
-  *out = counts[dev];
-  return cudaSuccess;
 }
 
 // CTAs that run at once: 16 warps an SM for the backward's registers, 32 for the

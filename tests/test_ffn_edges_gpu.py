@@ -95,3 +95,40 @@ def test_hidden_values_past_the_type(T, dtype):
     assert (on[:, :4] == float("inf")).all() and (on[:, 4:8] == -float("inf")).all()
     assert torch.isnan(on[:, 8:12]).all() and (on[:, 12:] == float("inf")).all()
     assert torch.isfinite(y[1::2]).all()
+
+
+def test_calls_from_many_threads_at_once():
+    """Every variant and both directions from four threads on streams of their own: the bits of
+    one thread's calls."""
+    import threading
+    from dsalt import counter_dropout, residual_norm
+    from dsalt.kernels.gated_ffn import gated_ffn
+    seed = torch.tensor([3], dtype=torch.int64, device="cuda")
+    ffn = [inputs(T, 264, 520, 264, torch.bfloat16) for T in (4, 30, 200, 700)]
+    x, f, w = (torch.randn(s, device="cuda").requires_grad_(True) for s in ((300, 777), (300, 777), (777,)))
+
+    def work():
+        out = []
+        for *leaves, dy in ffn:
+            y = gated_ffn(*leaves)
+            out += [y, *torch.autograd.grad(y, leaves, dy)]
+        x_new, h = residual_norm(counter_dropout(x, 0.25, seed, 1), f, w, post_weight=w, dropout_p=0.1, seed=seed)
+        return out + [x_new, h, *torch.autograd.grad((x_new.sum() + h.square().sum()), (x, f, w))]
+
+    ref = work()
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def thread(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i] = work()
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for out in got:
+        assert all(torch.equal(a, b) for a, b in zip(out, ref))
