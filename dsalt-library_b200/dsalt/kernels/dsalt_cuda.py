@@ -33,8 +33,8 @@ def device_status(device: torch.device) -> torch.Tensor:
     key = (device.type, device.index if device.index is not None else torch.cuda.current_device())
     st = _STATUS.get(key)
     if st is None:
-        st = torch.zeros(1, dtype=torch.int32, device=device)
-        _STATUS[key] = st
+        # of two threads' words the first stays
+        st = _STATUS.setdefault(key, torch.zeros(1, dtype=torch.int32, device=device))
     return st
 
 

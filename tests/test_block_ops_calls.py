@@ -82,3 +82,19 @@ def test_forward_mode_is_refused(launches, name, no_grad):
         del launches[:]
         fn(*args)
         assert len(launches) == 1
+
+
+def test_one_status_word_however_many_threads_make_it(monkeypatch):
+    """A thread that finds no status word may make one while another does: both get the word
+    that is kept, so that no launch holds the address of one that was freed."""
+    from dsalt.kernels import dsalt_cuda
+    monkeypatch.setattr(dsalt_cuda, "_STATUS", {})
+    zeros, other = torch.zeros, torch.zeros(1, dtype=torch.int32)
+
+    def zeros_while_another_thread_is_first(*args, device, **kw):
+        dsalt_cuda._STATUS[("cuda", 0)] = other
+        return zeros(*args, **kw)
+
+    monkeypatch.setattr(torch, "zeros", zeros_while_another_thread_is_first)
+    assert dsalt_cuda.device_status_ptr(torch.device("cuda:0")) == other.data_ptr()
+    assert dsalt_cuda._STATUS == {("cuda", 0): other}
