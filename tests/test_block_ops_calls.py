@@ -96,5 +96,5 @@ def test_one_status_word_however_many_threads_make_it(monkeypatch):
         return zeros(*args, **kw)
 
     monkeypatch.setattr(torch, "zeros", zeros_while_another_thread_is_first)
-    assert dsalt_cuda.device_status_ptr(torch.device("cuda:0")) == other.data_ptr()
+    assert dsalt_cuda.device_status(torch.device("cuda:0")) is other
     assert dsalt_cuda._STATUS == {("cuda", 0): other}
