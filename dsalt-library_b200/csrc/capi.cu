@@ -404,6 +404,9 @@ static int check_ffn(const DsaltGatedFfnParams* p, bool bwd) {
   // tile coordinates and counts are 32-bit
   const int64_t most = (int64_t)1 << 30;
   if (p->T > most || p->d > most || p->F > most || p->d_out > most) return DSALT_ERR_TOO_LARGE;
+  // the epilogue of a weight gradient's tile waits for all its products, up to 1150 cycles
+  // for 64 tokens: 2^27 tokens stay well inside a wait's limit of 4·10^9 cycles
+  if (bwd && p->T > (int64_t)1 << 27 && (p->dw_gate || p->dw_up || p->dw_down)) return DSALT_ERR_TOO_LARGE;
   const int64_t tall = p->T > p->F ? p->T : p->F, wide = p->d > p->d_out ? p->d : p->d_out;
   const int64_t cols = p->F > wide ? p->F : wide, rows = tall > wide ? tall : wide;
   if (((rows + 127) / 128) * ((cols + 127) / 128) > INT32_MAX / 4) return DSALT_ERR_TOO_LARGE;

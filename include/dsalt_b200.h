@@ -505,7 +505,8 @@ DSALT_API int dsalt_swiglu_bwd(const DsaltSwigluParams* p, void* stream);
  * what the set ones of dx, dw_gate, dw_up and dw_down need; the weight gradients in
  * dtype, or in fp32 with w_grad_f32.  Inputs and h, a, b, ab, dg, du: 16-byte aligned,
  * strides multiples of 8; in those five columns F up to the next multiple of 8 may be
- * written.  y, dx and the weight gradients are dense, of any alignment.      */
+ * written.  y, dx and the weight gradients are dense, of any alignment.  T up to
+ * 2^30, with weight gradients 2^27.                                            */
 #define DSALT_FFN_FEW_TOKENS 64
 enum { DSALT_ACT_SILU = 0, DSALT_ACT_GELU = 1, DSALT_ACT_GELU_TANH = 2 };
 typedef struct DsaltGatedFfnParams {

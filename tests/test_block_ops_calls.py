@@ -98,3 +98,27 @@ def test_one_status_word_however_many_threads_make_it(monkeypatch):
     monkeypatch.setattr(torch, "zeros", zeros_while_another_thread_is_first)
     assert dsalt_cuda.device_status(torch.device("cuda:0")) is other
     assert dsalt_cuda._STATUS == {("cuda", 0): other}
+
+
+def test_products_too_long_for_the_kernels_waits_are_refused():
+    """A tile's products all end before its epilogue starts, within the limit of the kernels'
+    waits (about 2 s): past 2^27 tokens a weight gradient is refused instead of given up on the
+    device.  (Widths are held far below by the number of tiles.)"""
+    import ctypes
+    from dsalt.kernels import _ext
+    align, large, lib = 6, 7, _ext.load()  # DSALT_ERR_*
+
+    def rc(name, **kw):
+        base = dict(x=16, w_gate=16, w_up=16, w_down=16, h=16, h_lo=16, y=16, dy=16, a=16, b=16, ab=16, dg=16, du=16,
+                    T=4, ld_x=64, ld_wg=64, ld_wu=64, ld_wd=96, ld_f=96, ld_dy=64, d=64, F=96, d_out=64, dtype=_ext.BF16)
+        return getattr(lib, name)(ctypes.byref(_ext.GatedFfnParams(**{**base, **kw})), ctypes.c_void_p(0))
+
+    for grad in ("dw_gate", "dw_up", "dw_down"):
+        assert rc("dsalt_gated_ffn_bwd", T=(1 << 27) + 1, **{grad: 16}) == large, grad
+        # refused for its pointers, not for its size (and so before any launch)
+        assert rc("dsalt_gated_ffn_bwd", T=1 << 27, dy=24, **{grad: 16}) == align, grad
+    assert rc("dsalt_gated_ffn_bwd", T=1 << 29, dy=24, dx=16) == align
+    assert rc("dsalt_gated_ffn_fwd", T=1 << 29, x=24) == align
+    n = (1 << 22) + 8
+    for wide in (dict(d=n, ld_x=n, ld_wg=n, ld_wu=n), dict(F=n, ld_wd=n, ld_f=n), dict(d_out=n, ld_dy=n)):
+        assert rc("dsalt_gated_ffn_fwd", **wide) == rc("dsalt_gated_ffn_bwd", dx=16, **wide) == large, wide
