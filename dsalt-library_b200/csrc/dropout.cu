@@ -1,6 +1,7 @@
 // Dropout whose mask is computed from (seed, site, element index) and never stored
 // (dropout.cuh): y = keep ? x·65536 / (65536 − threshold) : 0.  The backward is the
-// same pass over the gradient.  A dropped element is 0 whatever x holds there.
+// same pass over the gradient.  A dropped element is 0 whatever x holds there.  y may be x:
+// a thread reads its elements before it writes them, and not by the read-only path.
 // Bound: one read and one write of the tensor.
 #include "dropout.cuh"
 
@@ -36,7 +37,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DsaltDropoutPar
   if (VEC && first + ((kBlocks - 1) * kThreads + 1) * 8 <= p.n) {
     Raw<T, true> raw[kBlocks];
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b) raw[b].load(x + first + b * kThreads * 8, 8);
+    for (int b = 0; b < kBlocks; ++b) raw[b].load_in_place(x + first + b * kThreads * 8);
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
       drop(raw[b], first + b * kThreads * 8);

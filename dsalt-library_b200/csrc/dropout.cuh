@@ -141,12 +141,18 @@ struct Raw {
 template <typename T>
 struct Raw<T, true> {
   uint32_t w[2 * sizeof(T)];
+  // through the read-only path: no launch still running writes what it reads
   __device__ __forceinline__ void load(const T* p, int) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
-      w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
-    }
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) put(i, __ldg(reinterpret_cast<const uint4*>(p) + i));
+  }
+  // of what this thread writes next
+  __device__ __forceinline__ void load_in_place(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) put(i, reinterpret_cast<const uint4*>(p)[i]);
+  }
+  __device__ __forceinline__ void put(int i, uint4 u) {
+    w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll

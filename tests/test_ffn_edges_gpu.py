@@ -132,3 +132,15 @@ def test_calls_from_many_threads_at_once():
         t.join()
     for out in got:
         assert all(torch.equal(a, b) for a, b in zip(out, ref))
+
+
+@pytest.mark.parametrize("n", [8, 4099, 3_000_008])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_dropout_in_place(n, dtype):
+    """The C entry may write where it reads."""
+    from dsalt import counter_dropout
+    from dsalt.kernels import _ext
+    x, seed = torch.randn(n, device="cuda").to(dtype), torch.tensor([3], dtype=torch.int64, device="cuda")
+    ref = counter_dropout(x, 0.25, seed, 2)
+    _ext.call("dsalt_dropout", _ext.DropoutParams(_ext.ptr(x), _ext.ptr(x), _ext.ptr(seed), n, 2, 16384, _ext.dtype_code(dtype)))
+    assert torch.equal(x, ref)
