@@ -36,9 +36,13 @@ struct Dropout {
     const uint64_t s = threshold_ > 0 ? (uint64_t)__ldg(seed) : 0;
     key = make_uint2((uint32_t)s, (uint32_t)(s >> 32));
   }
+  // the draws of elements 8·block … 8·block + 7
+  __device__ __forceinline__ uint4 draws(uint64_t block) const {
+    return philox(make_uint4((uint32_t)block, (uint32_t)(block >> 32), site, 0u), key);
+  }
   // v, 8·block … 8·block + 7, with 0 where dropped
   __device__ __forceinline__ void select_block(uint64_t block, float* v) const {
-    const uint4 w = philox(make_uint4((uint32_t)block, (uint32_t)(block >> 32), site, 0u), key);
+    const uint4 w = draws(block);
     const uint32_t d[4] = {w.x, w.y, w.z, w.w};
     const uint32_t high = threshold << 16;
     const bool some = threshold < 65536;
@@ -50,7 +54,7 @@ struct Dropout {
   }
   // m[j] = all ones where element 8·block + j is kept, 0 where it is dropped
   __device__ __forceinline__ void masks_block(uint64_t block, uint32_t* m) const {
-    const uint4 w = philox(make_uint4((uint32_t)block, (uint32_t)(block >> 32), site, 0u), key);
+    const uint4 w = draws(block);
     const uint32_t v[4] = {w.x, w.y, w.z, w.w};
     if (threshold >= 65536) {
 #pragma unroll
