@@ -11,7 +11,7 @@ namespace ffn {
 
 // ½·erfc(z) for z ≥ 0 given e = exp(−z²): e·t·P(t), t = 1 / (1 + z/2), with P a
 // polynomial fitted to ½·erfcx(z) / t on t in (0, 1] (least squares in relative error at
-// Chebyshev points, own coefficients; largest relative error 6e-7).
+// Chebyshev points, own coefficients; largest relative error 4.5e-7, in fp32 arithmetic 6.9e-7).
 __device__ __forceinline__ float half_erfc(float z, float e) {
   const float t = sm100::fast_rcp(fmaf(0.5f, z, 1.f));
   float p = -0.0219386164f;
@@ -26,9 +26,11 @@ __device__ __forceinline__ float half_erfc(float z, float e) {
   return e * (t * p);
 }
 
-// act(g) and act'(g).  exp and the reciprocal are the fast ones (relative error
-// below 2^-20 over the range where the result is not rounded to 0 or g): the
-// results are rounded to 16 or 24 bits next.
+// act(g) and act'(g).  exp and the reciprocal are the fast ones.  Relative error of act
+// below 2^-19 for |g| <= 4 (silu 3e-7, gelu 1.1e-6, gelu_tanh 1.5e-6); towards −∞ it grows
+// with the exponent's argument, whose rounding in fp32 alone is 2^-24 of its size: 3.5e-6
+// for silu at −87, 7e-6 for gelu at −12 and 5e-6 for gelu_tanh at −9, the ends of bf16's
+// range.  The results are rounded to 16 or cut to 24 bits next (2^-8, 2^-15).
 template <int ACT>
 __device__ __forceinline__ void act_pair(float g, float& a, float& da) {
   constexpr float kLog2e = 1.4426950409f;

@@ -12,15 +12,18 @@
 //               also stores a = act(g) and b = u⊙act'(g), which is all the backward
 //               needs of g and u: du = dh⊙a and dg = dh⊙b need no exponential and do
 //               not depend on the activation.  a and b are kept to 24 bits (fp32
-//               without its last byte: two 16-bit words and a word of the two next
-//               bytes): rounded to 16 bits they would add a third rounding to dx, dWg
-//               and dWu beside those of dg or du and of the result (error against 64
-//               bits 1.73 roundings instead of 1.41);
+//               without its last byte, cut and not rounded, so up to 2^-15 of the value
+//               towards 0: two 16-bit words and a word of the two next bytes): rounded
+//               to 16 bits they would add a third rounding to dx, dWg and dWu beside
+//               those of dg or du and of the result (error against 64 bits 1.73
+//               roundings instead of 1.41);
 //   out, dx, dW the accumulator rounded once to the result's type;
 //   dhidden     dh stays in fp32 and is multiplied with the a and b tiles.
 // Bound: the tensor pipe (6·T·d·F flops forward, 12·T·d·F backward).  T = 16384,
-// d = 1024, F = 2816, bf16: 676 us of kernels for the step (1,257 TFLOP/s; 0.76 of the
-// measured burst rate), in a long loop 790 us at 1.35 to 1.5 GHz under the power cap.
+// d = 1024, F = 2816, bf16: 648 us of kernels for the step in a replayed graph (1,312
+// TFLOP/s; 0.80 of the measured burst rate), in a long loop 790 us at 1.35 to 1.5 GHz under
+// the power cap.  Where two times stand beside a choice below, both were taken at the step
+// that made it.
 //
 // A tile is 256 rows × BN columns worked on by a pair of CTAs (a cluster of 2,
 // cta_group::2): each holds 128 rows of A, half of B's columns and the accumulator of

@@ -2,15 +2,19 @@
 //   n  = f·rf·post (or f),  s = x + D(scale⊙gate⊙n),  x' = R(s),  h = R(s·r·norm)
 // with rf and r the inverse root mean squares of f and s, D the dropout of
 // dropout.cuh and R the rounding to the tensors' type: h is the norm of the sum
-// before its rounding, so that it is off by one rounding and not by two.  Backward,
-// from the stored x':
+// before its rounding, so that it is off by one rounding and not by two.  Backward, from
+// the stored x' (rounded, with r of the sum before: dnorm and the projection in G see that
+// rounding, a second one beside their own; s itself would be as many bytes again):
 //   G = dx_new + r·(dh⊙norm − x'·r²·mean(dh⊙norm⊙x')),  dx = R(G),  dn = D(G)⊙scale⊙gate,
 //   df = R(rf·(dn⊙post − f·rf²·mean(dn⊙post⊙f))),  dgate = D(G)⊙scale⊙n,
 //   dscale = Σ_t D(G)⊙gate⊙n,  dpost = Σ_t dn⊙f·rf,  dnorm = Σ_t dh⊙x'·r.
 // Everything between the loads and the stores is fp32.  Bound by the rows' bytes, once in
 // and once out, and with dropout by issue slots (the generator's ten rounds a block of
-// eight elements).  16384 × 1024 bf16 with every part: forward 41 us (29 without dropout;
-// 134 MB), backward 61 us (48; 201 MB).
+// eight elements).  16384 × 1024 bf16 with every part, in replayed graphs: forward 41 us (31
+// without dropout; 134 MB), backward with its column sums 65 us (53; 201 MB); fp32 forward
+// 54 us (52), backward 76 us (72).  Under the profiler the bf16 kernels issue in 50 to 55 %
+// of the cycles and use a quarter to two fifths of DRAM's rate: neither is full, the rest is
+// latency, with 23 % (backward) and 43 % of an SM's warps resident.
 //
 // A row belongs to a group of threads of eight consecutive columns each: 8, 16 or
 // 32 lanes of a warp up to d = 256, else a whole CTA (of one, two or four chunks of
@@ -43,8 +47,9 @@ struct Shape {
   int chunks;  // 8-column chunks of a thread
 };
 // Two chunks a thread past d = 4096, and from d = 512 on where rows are read element by
-// element (16384 × 1001 bf16: 229 us instead of 276 with one); one elsewhere (16384 × 1024:
-// 109 us instead of 117 with two, before the forward selected instead of masking).
+// element (16384 × 1001 bf16: 229 us instead of 276 with one, both before masks were shifted
+// bits; 200 now); one elsewhere (16384 × 1024: 109 us instead of 117 with two, both before
+// the forward selected instead of masking; 106 now).
 inline Shape shape_of(int d, bool vec) {
   const int units = (d + 7) / 8;
   if (units <= 8) return {8, kSmallThreads, 1};

@@ -8,7 +8,7 @@ needs gradients also keeps ``a = act(g)`` and ``b = u·act'(g)``, from which the
 backward forms ``du = dh·a`` and ``dg = dh·b`` in the epilogue of the product that
 makes ``dh``.  Results are rounded once from the fp32 sums; on the way only the
 operands of a further product are rounded to 16 bits, ``h``, ``dg`` and ``du``
-(``a`` and ``b`` are kept to 24 bits, and ``h`` to two words in a forward of few tokens).
+(``a`` and ``b`` are cut to 24 bits, and ``h`` to two words in a forward of few tokens).
 
 ``swiglu_ffn`` computes the same block with library GEMMs around an activation
 kernel, with torch's rounding at every step.

@@ -498,7 +498,7 @@ DSALT_API int dsalt_swiglu_bwd(const DsaltSwigluParams* p, void* stream);
  * the second product takes h to two 16-bit words (h + h_lo) and is not off by h's
  * rounding.  The forward writes y, h (rounded once from
  * fp32) and, with a, b and ab set, what a backward needs of g and u: a = act(g) and
- * b = u⊙act'(g) as the upper 24 bits of their fp32 values, the upper 16 in a and b,
+ * b = u⊙act'(g) as the upper 24 bits of their fp32 values (cut), the upper 16 in a and b,
  * the next 8 of each in the low and high byte of ab.  The backward forms, of
  *   dh = dy·Wd (kept in fp32), du = R(dh⊙a), dg = R(dh⊙b), dx = R(dg·Wg + du·Wu),
  *   dWg = dgᵀ·x, dWu = duᵀ·x, dWd = dyᵀ·h,
